@@ -390,6 +390,118 @@ int32_t kvq_sdpa_decode_noalloc(const kvq_qtensor* keys, const kvq_qtensor* valu
                                 const void* q, int32_t q_heads, float scale,
                                 const int32_t* seq_lens, void* out, void* stream);
 
+/* ---- paged quantized cache ---------------------------------------------- */
+
+/* A pool of pages shared by many sequences, in the caches' affine quantized
+ * format, and the operators that fill and read it.  No counterpart in the
+ * reference, whose caches are contiguous per sequence.
+ *
+ * The pool is caller-owned device memory [num_pages][kv_heads][page_size /
+ * 16] tiles of kvq_paged_tile_bytes bytes.  A tile is 16 consecutive token
+ * rows of one kv head, all of its parts contiguous:
+ *   K codes [16][head_dim * bits / 32] uint32 (the packing of kvq_qtensor),
+ *   K (scale, bias) pairs [16][head_dim / group_size][2] dtype,
+ *   V codes, V pairs likewise.
+ * A page is one contiguous run of bytes, so it is copied, shared between
+ * sequences or moved to the host as one block. */
+typedef struct kvq_paged {
+  void* pool;           /* 16-byte aligned */
+  int32_t* status;      /* device int32, zeroed by the caller at creation: error flag */
+  int32_t num_pages;
+  int32_t page_size;    /* token rows per page: 16, 32, 64, 128 or 256 */
+  int32_t kv_heads;
+  int32_t head_dim;     /* 64, 128 or 256 */
+  int32_t bits;         /* 4 or 8 */
+  int32_t group_size;   /* 32, 64 or 128, at most head_dim */
+  int32_t dtype;        /* KVQ_DTYPE_FLOAT16 or KVQ_DTYPE_BFLOAT16 */
+  int32_t device;
+} kvq_paged;
+
+/* One step of a batch, all arrays on the device: the same description serves
+ * the append and the attention of the step.
+ *   page_table [batch] rows of max_pages int32, table_stride elements apart:
+ *     token position p of sequence b lies in page page_table[b][p /
+ *     page_size].  Entries behind a sequence's last page are not read.
+ *   seq_lens [batch]: tokens of each sequence, this step's rows included.
+ *   cu_rows [batch + 1]: sequence b owns rows [cu_rows[b], cu_rows[b + 1]) of
+ *     the step's q / k / v; ascending.  NULL: one row per sequence (rows =
+ *     batch).
+ *   rows: token rows of the q / k / v buffers.  Rows from cu_rows[batch] on
+ *     are padding: neither read nor written.
+ * Row j of the n rows of sequence b stands at position seq_lens[b] - n + j.
+ * Positions, lengths and pages are read when the kernels run, so a captured
+ * graph takes the values that the arrays hold at each replay.  A row whose
+ * position is negative or has no page, a page number outside [0, num_pages)
+ * and a length beyond max_pages * page_size raise the pool's error flag
+ * (kvq_paged_check); the row is skipped, or reads as if the key were masked. */
+typedef struct kvq_paged_batch {
+  const int32_t* page_table;
+  int64_t table_stride;
+  const int32_t* seq_lens;
+  const int32_t* cu_rows;
+  int32_t batch;
+  int32_t max_pages;
+  int32_t rows;
+} kvq_paged_batch;
+
+/* Rotary embedding: the first `dims` elements of a row turn in pairs (i, i +
+ * dims / 2), or (2i, 2i + 1) when traditional, by (scale * position) *
+ * inv_freq_i, inv_freq_i = base^(-2i / dims) or 1 / freqs[i] (device f32 [dims
+ * / 2]; an infinite entry leaves its pair in place), and are multiplied by
+ * pre_scale.  Angles and rotation are computed in 64 bits and the result is
+ * rounded to 32 and then to the dtype, so far positions keep their precision
+ * (kvq_append_projected follows MLX's 32-bit angles instead). */
+typedef struct kvq_rope {
+  int32_t dims;         /* even, within head_dim; 0: no rotation */
+  int32_t traditional;
+  float base;
+  float scale;          /* 0: 1 */
+  float pre_scale;      /* 0: 1 */
+  const float* freqs;   /* nullable */
+} kvq_rope;
+
+/* Bytes of one 16-row tile of the pool. */
+int32_t kvq_paged_tile_bytes(const kvq_paged* cache, size_t* bytes);
+
+/* Write the step's rows into their pages: K rotated at its position, K and V
+ * quantized by the rule of kvq_append (same codes).  k, v: device [rows,
+ * kv_heads, head_dim] dtype with element strides (row, head); the element
+ * stride is 1.  q (nullable): device [rows, q_heads, head_dim] with its own
+ * strides, whose rotated rows go to q_out (contiguous [rows, q_heads,
+ * head_dim], or q itself when q is contiguous).  rope NULL: no rotation.  Two
+ * rows of one step must not share a position of one page. */
+int32_t kvq_paged_append(const kvq_paged* cache, const kvq_paged_batch* batch, const void* k,
+                         const void* v, const int64_t* k_strides, const int64_t* v_strides,
+                         const kvq_rope* rope, const void* q, int32_t q_heads,
+                         const int64_t* q_strides, void* q_out, void* stream);
+
+/* Causal attention of the step's query rows over their sequences' pages.
+ * q: device [rows, q_heads, head_dim] with element strides (row, head); out:
+ * contiguous [rows, q_heads, head_dim]; query head h uses kv head h / (q_heads
+ * / kv_heads).  A query at position p sees key j when j <= p and (window == 0
+ * or j > p - window or j < sinks): a sliding window with the first `sinks`
+ * tokens kept visible.  A row that sees no key gives zeros.  k and v are code
+ * * scale + bias, logits and softmax are f32, the output is rounded once.
+ * kvq_paged_sdpa_decode takes one row per sequence (cu_rows is not read,
+ * rows = batch); kvq_paged_sdpa_prefill takes ragged rows.
+ * workspace: device memory of kvq_paged_sdpa_workspace bytes (16-byte
+ * aligned, contents irrelevant) that no other call uses meanwhile; NULL: the
+ * call takes and returns its own, stream-ordered (cudaMallocAsync), so calls
+ * on several streams and captured graphs share nothing. */
+int32_t kvq_paged_sdpa_workspace(const kvq_paged* cache, const kvq_paged_batch* batch,
+                                 int32_t q_heads, int32_t decode, size_t* bytes);
+int32_t kvq_paged_sdpa_decode(const kvq_paged* cache, const kvq_paged_batch* batch, const void* q,
+                              int32_t q_heads, const int64_t* q_strides, float scale,
+                              int32_t window, int32_t sinks, void* out, void* workspace,
+                              size_t workspace_bytes, void* stream);
+int32_t kvq_paged_sdpa_prefill(const kvq_paged* cache, const kvq_paged_batch* batch,
+                               const void* q, int32_t q_heads, const int64_t* q_strides,
+                               float scale, int32_t window, int32_t sinks, void* out,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* Synchronize `stream`, report (then clear) the pool's error flag. */
+int32_t kvq_paged_check(const kvq_paged* cache, void* stream);
+
 /* ---- context split across the GPUs of one node (peer memory) ----------- */
 
 /* Exchange of context-split partials among the nranks ranks (one process

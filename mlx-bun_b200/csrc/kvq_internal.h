@@ -22,6 +22,20 @@ int32_t cuda_fail(cudaError_t e, const char* what);
     if (_e != cudaSuccess) return ::kvq::cuda_fail(_e, #expr); \
   } while (0)
 
+// Selects a device for the life of the guard.
+struct DeviceGuard {
+  int prev = -1;
+  bool ok = true;
+  explicit DeviceGuard(int dev) {
+    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+    if (prev != dev) ok = cudaSetDevice(dev) == cudaSuccess;
+  }
+  ~DeviceGuard() {
+    int cur = -1;
+    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
+  }
+};
+
 // Geometry of one quantized row.
 struct RowGeom {
   int D, bits, gs;

@@ -30,7 +30,9 @@ EXPORTS = (
     "kvq_peer_group_connect", "kvq_peer_exchange_merge", "kvq_peer_group_check",
     "kvq_peer_group_free", "kvq_append_ragged", "kvq_cache_fetch_all", "kvq_cache_check",
     "kvq_cache_from_dense", "kvq_cache_export", "kvq_cache_import", "kvq_append_projected",
-    "kvq_append_projected_workspace",
+    "kvq_append_projected_workspace", "kvq_paged_tile_bytes", "kvq_paged_append",
+    "kvq_paged_sdpa_workspace", "kvq_paged_sdpa_decode", "kvq_paged_sdpa_prefill",
+    "kvq_paged_check",
 )
 
 
@@ -71,6 +73,27 @@ class KvProjection(ctypes.Structure):
                 ("rope_scale", ctypes.c_float), ("rope_pre_scale", ctypes.c_float),
                 ("rope_freqs", ctypes.c_void_p), ("q_proj", QLinear), ("q_heads", ctypes.c_int32),
                 ("q_norm", ctypes.c_int32), ("q_norm_weight", ctypes.c_void_p)]
+
+
+class Paged(ctypes.Structure):
+    """kvq_paged: a pool of pages."""
+    _fields_ = [("pool", ctypes.c_void_p), ("status", ctypes.c_void_p)] + \
+        [(n, ctypes.c_int32) for n in ("num_pages", "page_size", "kv_heads", "head_dim", "bits",
+                                       "group_size", "dtype", "device")]
+
+
+class PagedBatch(ctypes.Structure):
+    """kvq_paged_batch: one step's sequences and rows."""
+    _fields_ = [("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("seq_lens", ctypes.c_void_p), ("cu_rows", ctypes.c_void_p)] + \
+        [(n, ctypes.c_int32) for n in ("batch", "max_pages", "rows")]
+
+
+class RopeArgs(ctypes.Structure):
+    """kvq_rope: rotary embedding of the paged append."""
+    _fields_ = [("dims", ctypes.c_int32), ("traditional", ctypes.c_int32),
+                ("base", ctypes.c_float), ("scale", ctypes.c_float),
+                ("pre_scale", ctypes.c_float), ("freqs", ctypes.c_void_p)]
 
 
 _lib = None
@@ -126,6 +149,16 @@ def lib():
                                        ctypes.c_size_t, vp]),
         "kvq_append_projected_workspace": (i32, [vp, i32, P(KvProjection),
                                                  P(ctypes.c_size_t)]),
+        "kvq_paged_tile_bytes": (i32, [P(Paged), P(ctypes.c_size_t)]),
+        "kvq_paged_append": (i32, [P(Paged), P(PagedBatch), vp, vp, P(i64), P(i64), P(RopeArgs),
+                                   vp, i32, P(i64), vp, vp]),
+        "kvq_paged_sdpa_workspace": (i32, [P(Paged), P(PagedBatch), i32, i32,
+                                           P(ctypes.c_size_t)]),
+        "kvq_paged_sdpa_decode": (i32, [P(Paged), P(PagedBatch), vp, i32, P(i64), f32, i32, i32,
+                                        vp, vp, ctypes.c_size_t, vp]),
+        "kvq_paged_sdpa_prefill": (i32, [P(Paged), P(PagedBatch), vp, i32, P(i64), f32, i32, i32,
+                                         vp, vp, ctypes.c_size_t, vp]),
+        "kvq_paged_check": (i32, [P(Paged), vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
