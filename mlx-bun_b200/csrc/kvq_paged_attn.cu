@@ -1,125 +1,87 @@
-// kvq_paged_attn.cu — causal attention of ragged query rows over the pages
-// (sliding window and sinks), the plain form: one block per (token row, query
-// head), each warp takes every fourth visible key, lanes share the row.
-#include "kvq_paged.cuh"
+// kvq_paged_attn.cu — host side of the attention over pages: which kernel, its
+// workspace and its launches.
+#include <algorithm>
+
+#include "kvq_paged_cols.cuh"
 
 namespace kvq {
 namespace paged {
+
+template <>
+int32_t launch_cols<4, false>(const AttnArgs&, const Work&, int, int, int, cudaStream_t);
+template <>
+int32_t launch_cols<4, true>(const AttnArgs&, const Work&, int, int, int, cudaStream_t);
+template <>
+int32_t launch_cols<8, false>(const AttnArgs&, const Work&, int, int, int, cudaStream_t);
+template <>
+int32_t launch_cols<8, true>(const AttnArgs&, const Work&, int, int, int, cudaStream_t);
+
 namespace {
 
-constexpr int kWarps = 4;
-constexpr float kNegInf = -3.0e38f;
+size_t up16(size_t x) { return (x + 15) / 16 * 16; }
 
-template <bool BF>
-__device__ __forceinline__ float to_f(uint32_t v) {
-  if constexpr (BF) return __uint_as_float(v << 16);
-  else return __half2float(__ushort_as_half((uint16_t)v));
-}
+// The column kernel's launch: columns per block, CTAs and workspace layout.
+struct ColsLaunch {
+  int NC, ctas;
+  long long max_blocks;
+  bool big;  // the plan does not fit in shared memory
+  size_t o_meta, o_gpre, o_tpre, o_ng, bytes;
+};
 
-// This lane's PER elements of one K or V row
-template <bool BF, int BITS, int PER>
-__device__ __forceinline__ void row_values(float (&x)[PER], const uint8_t* half, int row, int e0,
-                                           int crb, int gs, int prb) {
-  const uint32_t pr = *reinterpret_cast<const uint32_t*>(half + kTileRows * crb + row * prb + e0 / gs * 4);
-  const float s = to_f<BF>(pr & 0xffffu), z = to_f<BF>(pr >> 16);
-#pragma unroll
-  for (int i = 0; i < PER; i++) {
-    const int bit = (e0 + i) * BITS;
-    const uint8_t byte = half[row * crb + bit / 8];
-    const int c = BITS == 8 ? byte : (byte >> (bit & 4)) & 15;
-    x[i] = fmaf((float)c, s, z);
-  }
-}
-
-template <bool BF, int BITS, int PER>
-__global__ void __launch_bounds__(kWarps * 32) attn_rows_kernel(const AttnArgs a) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int D = 32 * PER;
-  __shared__ float sm[kWarps], sl[kWarps], so[kWarps][D];
+ColsLaunch cols_launch(const AttnArgs& a) {
+  ColsLaunch c{};
   const View& v = a.v;
-  const int t = blockIdx.x, h = blockIdx.y, hk = h / a.rep;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, e0 = lane * PER;
-  const int b = block_find_seq(v, t);
-  if (b >= v.B) return;
-  int row0, n, len;
-  seq_rows(v, b, row0, n, len);
-  int pos = len - n + (t - row0);
-  if (t < row0 || len < 0 || len > (int64_t)v.max_pages << v.page_shift) {
-    if (threadIdx.x == 0) raise(v);
-    pos = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&c.ctas, cudaDevAttrMultiProcessorCount, dev);
+  // columns per block: 16 where a sequence has more than 8 (K and V are read
+  // once for all; D 256 has no registers for them), 4 where it has no more
+  const long long cols = (long long)v.rows * a.rep;
+  c.NC = cols > 8ll * v.B ? (v.D < 256 ? 16 : 8) : (cols > 4ll * v.B ? 8 : 4);
+  const int NC = c.NC, NT = NC > 8 ? 2 : 1;
+  c.max_blocks = v.cu ? cols / NC + v.B : (long long)v.B * ((a.rep + NC - 1) / NC);
+  c.big = v.B > kPlanMax || c.max_blocks > kPlanMax;
+  const size_t piece = (size_t)(16 * NT + v.D / 16 * NT * 128) * 4;
+  c.o_meta = 2 * (size_t)c.ctas * piece;
+  c.o_gpre = c.o_meta + (size_t)c.ctas * 16;
+  c.bytes = c.o_gpre;
+  if (c.big) {
+    c.o_tpre = up16(c.o_gpre + (size_t)(v.B + 1) * 4);
+    c.o_ng = c.o_tpre + (size_t)(c.max_blocks + 1) * 8;
+    c.bytes = up16(c.o_ng + 4);
   }
-  int lo = 0, head = 0;
-  if (a.window > 0) {
-    lo = max(0, pos - a.window + 1);
-    head = min(a.sinks, lo);
-  }
-  float q[PER], o[PER] = {};
-  const uint16_t* qr = a.q + (int64_t)t * a.q_row + (int64_t)h * a.q_head + e0;
-#pragma unroll
-  for (int i = 0; i < PER; i++) q[i] = to_f<BF>(qr[i]) * a.scale;
-  float m = kNegInf, l = 0.0f;
-  const int crb = code_row_bytes(D, BITS), prb = pair_row_bytes(D, v.gs);
-  const int keys = pos < 0 ? 0 : head + pos + 1 - lo;
-  for (int i = w; i < keys; i += kWarps) {
-    const int j = i < head ? i : lo + i - head;
-    const int page = v.table[(int64_t)b * v.table_stride + (j >> v.page_shift)];
-    if (page < 0 || page >= v.num_pages) {
-      if (lane == 0) raise(v);
-      continue;
-    }
-    const uint8_t* tile = tile_ptr(v, page, hk, (j & v.page_mask) >> 4);
-    float x[PER];
-    row_values<BF, BITS, PER>(x, tile, j & 15, e0, crb, v.gs, prb);
-    float s = 0.0f;
-#pragma unroll
-    for (int k = 0; k < PER; k++) s = fmaf(q[k], x[k], s);
-#pragma unroll
-    for (int k = 16; k; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-    const float m2 = fmaxf(m, s), f = expf(m - m2), p = expf(s - m2);
-    m = m2;
-    l = l * f + p;
-    row_values<BF, BITS, PER>(x, tile + kTileRows * (crb + prb), j & 15, e0, crb, v.gs, prb);
-#pragma unroll
-    for (int k = 0; k < PER; k++) o[k] = fmaf(p, x[k], o[k] * f);
-  }
-  if (lane == 0) sm[w] = m, sl[w] = l;
-#pragma unroll
-  for (int i = 0; i < PER; i++) so[w][e0 + i] = o[i];
-  __syncthreads();
-  float mx = sm[0];
-  for (int i = 1; i < kWarps; i++) mx = fmaxf(mx, sm[i]);
-  float lt = 0.0f;
-  for (int i = 0; i < kWarps; i++) lt += sl[i] * expf(sm[i] - mx);
-  for (int e = threadIdx.x; e < D; e += kWarps * 32) {
-    float s = 0.0f;
-    for (int i = 0; i < kWarps; i++) s += so[i][e] * expf(sm[i] - mx);
-    s = lt > 0.0f ? s / lt : 0.0f;
-    uint16_t r;
-    if constexpr (BF) r = __bfloat16_as_ushort(__float2bfloat16_rn(s));
-    else r = __half_as_ushort(__float2half_rn(s));
-    a.out[((int64_t)t * a.Hq + h) * D + e] = r;
-  }
+  return c;
 }
 
-template <bool BF, int BITS>
-int32_t dispatch(const AttnArgs& a, cudaStream_t st) {
-  const dim3 grid((unsigned)a.v.rows, (unsigned)a.Hq), block(kWarps * 32);
-  switch (a.v.D) {
-    case 64: KVQ_CUDA_TRY(launch_pdl(attn_rows_kernel<BF, BITS, 2>, grid, block, 0, st, a)); break;
-    case 128: KVQ_CUDA_TRY(launch_pdl(attn_rows_kernel<BF, BITS, 4>, grid, block, 0, st, a)); break;
-    default: KVQ_CUDA_TRY(launch_pdl(attn_rows_kernel<BF, BITS, 8>, grid, block, 0, st, a)); break;
-  }
-  return KVQ_OK;
+bool vec_ok(const AttnArgs& a) {
+  return reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_row % 8 == 0 && a.q_head % 8 == 0;
 }
 
 }  // namespace
 
-size_t paged_attn_workspace(const AttnArgs&) { return 0; }
+size_t paged_attn_workspace(const AttnArgs& a) { return cols_launch(a).bytes; }
 
-int32_t launch_paged_attn(const AttnArgs& a, void*, size_t, cudaStream_t st) {
-  if (a.v.bits == 4) return a.bf16 ? dispatch<true, 4>(a, st) : dispatch<false, 4>(a, st);
-  return a.bf16 ? dispatch<true, 8>(a, st) : dispatch<false, 8>(a, st);
+int32_t launch_paged_attn(const AttnArgs& a, void* ws, size_t, cudaStream_t st) {
+  const ColsLaunch c = cols_launch(a);
+  if (c.max_blocks * a.v.Hkv > 0x7fffffff) return fail(KVQ_ERR_ARG, "paged: too many rows * heads in one call");
+  uint8_t* p = static_cast<uint8_t*>(ws);
+  Work w{};
+  w.slots = reinterpret_cast<float*>(p);
+  w.meta = reinterpret_cast<int4*>(p + c.o_meta);
+  if (c.big) {
+    w.gpre = reinterpret_cast<int*>(p + c.o_gpre);
+    w.tpre = reinterpret_cast<long long*>(p + c.o_tpre);
+    w.ng = reinterpret_cast<int*>(p + c.o_ng);
+  }
+  w.max_blocks = (int)c.max_blocks;
+  w.vec = vec_ok(a);
+  int dev = 0;
+  KVQ_CUDA_TRY(cudaGetDevice(&dev));
+  if (a.v.bits == 4)
+    return a.bf16 ? launch_cols<4, true>(a, w, c.NC, c.ctas, dev, st)
+                  : launch_cols<4, false>(a, w, c.NC, c.ctas, dev, st);
+  return a.bf16 ? launch_cols<8, true>(a, w, c.NC, c.ctas, dev, st)
+                : launch_cols<8, false>(a, w, c.NC, c.ctas, dev, st);
 }
 
 }  // namespace paged

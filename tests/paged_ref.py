@@ -37,15 +37,20 @@ class RefPool:
         return table[pos // self.page].long(), (pos % self.page) // TILE, pos % TILE
 
     def rows(self, table, pos):
-        """K and V at positions `pos` of one sequence, f64 [n, heads, d]."""
+        """K and V at positions `pos` of one sequence, f64 [n, heads, d], and
+        what their rounding errors go by: |s| c + |z| of K and |s| max(c, top -
+        c) of V, for v = s c + z with codes up to `top`."""
         pg, tile, row = self.index(table, pos)
         shift = torch.arange(0, 32, self.bits, dtype=torch.int32)
-        out = []
+        out, top = [], float((1 << self.bits) - 1)
         for codes, pairs in ((self.kc, self.kp), (self.vc, self.vp)):
             c = (codes[pg, :, tile, row][..., None] >> shift) & ((1 << self.bits) - 1)
             c = c.flatten(-2).double().unflatten(-1, (self.g, self.gs))
             p = pairs[pg, :, tile, row].double()
+            a = p[..., :1].abs()
             out.append((c * p[..., :1] + p[..., 1:]).flatten(-2))
+            out.append((a * c + p[..., 1:].abs() if len(out) < 2 else
+                        a * torch.maximum(c, top - c)).flatten(-2))
         return out
 
     def put(self, table, pos, k, v):
@@ -86,54 +91,62 @@ def rotate(x, pos, dims, base=10000.0, scale=1.0, traditional=False, freqs=None,
 
 
 def attention(ref, q, table, lens, cu, scale, window=0, sinks=0):
-    """f64 outputs [rows, heads, d] and the two magnitudes that the tolerance
-    counts: sum_j p_j |v_j| per element, and the largest sum_d |q_d k_jd| *
-    scale over the visible keys per row and head."""
+    """f64 outputs [rows, heads, d] and the magnitudes that the tolerance
+    counts: sum_j p_j |v_j| and sum_j p_j |s_j| max(c_j, top - c_j) per
+    element, and the largest sum_d |q_d| (|s| c + |z|)_jd * scale over the
+    visible keys per row and head."""
     T, Hq, d = q.shape
     rep = Hq // ref.heads
     out = torch.zeros(T, Hq, d, dtype=torch.float64)
-    mag, l1 = torch.zeros_like(out), torch.zeros(T, Hq, 1, dtype=torch.float64)
+    mag, magc = torch.zeros_like(out), torch.zeros_like(out)
+    l1 = torch.zeros(T, Hq, 1, dtype=torch.float64)
     q = q.double()
     for b, n in enumerate(lens):
         r0, r1 = cu[b], cu[b + 1]
         if r1 <= r0 or n <= 0:
             continue
-        k, v = ref.rows(table[b], torch.arange(n))
+        k, ka, v, va = ref.rows(table[b], torch.arange(n))
         qpos = torch.arange(n - (r1 - r0), n)[:, None]
         j = torch.arange(n)[None]
         see = j <= qpos
         if window > 0:
             see &= (j > qpos - window) | (j < sinks)
         for h in range(Hq):
-            kk, vv = k[:, h // rep], v[:, h // rep]
-            s = (q[r0:r1, h] @ kk.T * scale).masked_fill(~see, float("-inf"))
+            g = h // rep
+            s = (q[r0:r1, h] @ k[:, g].T * scale).masked_fill(~see, float("-inf"))
             some = see.any(1)
             e = torch.exp(s - s.amax(1, keepdim=True).nan_to_num(neginf=0.0))
             p = torch.where(see, e, 0.0) / e.sum(1, keepdim=True).clamp_min(1e-300)
             p[~some] = 0
-            out[r0:r1, h] = p @ vv
-            mag[r0:r1, h] = p @ vv.abs()
-            a = (q[r0:r1, h].abs() @ kk.abs().T * scale).masked_fill(~see, 0.0)
+            out[r0:r1, h] = p @ v[:, g]
+            mag[r0:r1, h] = p @ v[:, g].abs()
+            magc[r0:r1, h] = p @ va[:, g]
+            a = (q[r0:r1, h].abs() @ ka[:, g].T * scale).masked_fill(~see, 0.0)
             l1[r0:r1, h] = a.amax(1, keepdim=True)
-    return out, mag, l1
+    return out, mag, magc, l1
 
 
-def tolerance(out, mag, l1, dt, dense):
+def tolerance(out, mag, magc, l1, dt, dense):
     """How far a kernel may be from the exact output.
 
-    Codes times fp16 (dense false, the single-token kernel): the output's own
-    rounding; the probabilities, with V's scale folded in, rounded to fp16
-    before their product with V, and ex2 and sums in f32 well within two more
-    such steps: 3 half steps of sum p |v|; logits in f32, an error of d 2^-24
-    of sum |q k|, 2^-16 for d = 256, moving the probabilities of both sums
-    (factor 2).  dense (the chunk kernel): probabilities, K and V are
-    rounded to the dtype before their products: a half step of the dtype
-    instead of fp16's, one more for V, and one of sum |q k| for K."""
-    u = half_step(dt) if dense else U16
-    logit = 2.0 ** -16 + (u if dense else 0.0)
-    rel = (4 if dense else 3) * u + 2 * logit * l1
-    floor = 6e-8 if dt == torch.float16 else 0.0  # fp16's subnormal step
-    return half_step(dt) * out.abs() * (1 + rel) + rel * mag + floor
+    Every output is rounded once: half a step of it.  Probabilities carry the
+    error of a logit summed in f32 over scales times codes, taken as 2^-18 of
+    sum |q| (|s| c + |z|) (16 partial sums and the two folds are some 20
+    roundings of 2^-24; 2^-18 is three times that), and ex2's 2^-20; it enters
+    the sums above and below the line: 2 of them, times sum p |v|.
+
+    The column kernel rounds p s to fp16, which multiplies c (bf16 outputs) or
+    c minus the middle code (fp16 outputs); both are at most max(c, top - c):
+    half a step of fp16, and 2^-18 for the f32 sums of s c + z, of magc.
+
+    dense: the chunk kernel may have run instead, which rounds p, K and V to
+    the dtype before their products: two half steps of sum p |v|, and one of
+    the logit's sum."""
+    u = half_step(dt) if dense else 0.0
+    p = (2.0 ** -18 + u) * l1 + 2.0 ** -20
+    err = (2 * p + 2 * u) * mag + (U16 + 2.0 ** -18) * magc
+    floor = 3e-8 if dt == torch.float16 else 0.0  # half of fp16's subnormal step
+    return half_step(dt) * (out.abs() + err) + err + floor
 
 
 def random_pool(gen, pages, page, heads, d, gs, bits, dt):

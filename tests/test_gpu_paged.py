@@ -35,11 +35,12 @@ def _pages(lens, page):
     return sum(-(-max(n, 0) // page) for n in lens) + 3
 
 
-def _check(got, want, mag, l1, dt, dense=False):
+def _check(got, want, mag, magc, l1, dt, dense=False):
     d = (got.double().cpu() - want).abs()
-    tol = R.tolerance(want, mag, l1, dt, dense)
+    tol = R.tolerance(want, mag, magc, l1, dt, dense)
     bad = d > tol
-    assert not bad.any(), (int(bad.sum()), float((d / tol).max()))
+    if bool(bad.any()):
+        raise AssertionError(f"{int(bad.sum())} outside, up to {float((d / tol).max()):.3f} times")
     assert bool(torch.isfinite(got).all())
 
 
