@@ -486,8 +486,9 @@ int32_t kvq_paged_append(const kvq_paged* cache, const kvq_paged_batch* batch, c
  * rows = batch); kvq_paged_sdpa_prefill takes ragged rows.
  * workspace: device memory of kvq_paged_sdpa_workspace bytes (16-byte
  * aligned, contents irrelevant) that no other call uses meanwhile; NULL: the
- * call takes and returns its own, stream-ordered (cudaMallocAsync), so calls
- * on several streams and captured graphs share nothing. */
+ * call takes and returns its own, stream-ordered (cudaMallocFromPoolAsync, from
+ * a pool of the library's), so calls on several streams and captured graphs
+ * share nothing. */
 int32_t kvq_paged_sdpa_workspace(const kvq_paged* cache, const kvq_paged_batch* batch,
                                  int32_t q_heads, int32_t decode, size_t* bytes);
 int32_t kvq_paged_sdpa_decode(const kvq_paged* cache, const kvq_paged_batch* batch, const void* q,

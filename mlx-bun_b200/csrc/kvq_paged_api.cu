@@ -1,6 +1,7 @@
 // kvq_paged_api.cu — C entry points of the paged quantized cache: argument
 // checks, workspaces, launches.  Nothing here throws: the arguments are plain
 // values and the only allocation is the stream-ordered workspace.
+#include <mutex>
 #include <string>
 
 #include "kvq_paged.cuh"
@@ -65,6 +66,31 @@ int32_t make_attn(const kvq_paged* c, const kvq_paged_batch* b, int32_t q_heads,
   return KVQ_OK;
 }
 
+// The library's own stream-ordered pool on `dev` (the current device) for
+// workspaces of calls that bring none.  Memory stays in it: the default pool
+// gives it back to the driver at every synchronization, and taking it again
+// costs hundreds of microseconds.
+std::mutex g_pool_mu;
+cudaMemPool_t g_pool[64] = {};
+
+int32_t scratch_pool(int dev, cudaMemPool_t* out) {
+  if (dev < 0 || dev >= 64) return fail(KVQ_ERR_ARG, "device ordinal out of range");
+  std::lock_guard<std::mutex> lk(g_pool_mu);
+  if (!g_pool[dev]) {
+    cudaMemPoolProps props = {};
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = dev;
+    cudaMemPool_t pool = nullptr;
+    KVQ_CUDA_TRY(cudaMemPoolCreate(&pool, &props));
+    uint64_t keep = UINT64_MAX;
+    KVQ_CUDA_TRY(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep));
+    g_pool[dev] = pool;
+  }
+  *out = g_pool[dev];
+  return KVQ_OK;
+}
+
 int32_t sdpa(const kvq_paged* c, const kvq_paged_batch* b, bool decode, const void* q,
              int32_t q_heads, const int64_t* q_strides, float scale, int32_t window, int32_t sinks,
              void* out, void* workspace, size_t workspace_bytes, void* stream) {
@@ -93,7 +119,9 @@ int32_t sdpa(const kvq_paged* c, const kvq_paged_batch* b, bool decode, const vo
   }
   if (!need) return paged::launch_paged_attn(a, nullptr, 0, st);
   void* ws = nullptr;
-  KVQ_CUDA_TRY(cudaMallocAsync(&ws, need, st));
+  cudaMemPool_t pool = nullptr;
+  if ((rc = scratch_pool(c->device, &pool))) return rc;
+  KVQ_CUDA_TRY(cudaMallocFromPoolAsync(&ws, need, pool, st));
   rc = paged::launch_paged_attn(a, ws, need, st);
   const cudaError_t e = cudaFreeAsync(ws, st);
   if (!rc && e != cudaSuccess) return cuda_fail(e, "cudaFreeAsync(paged workspace)");

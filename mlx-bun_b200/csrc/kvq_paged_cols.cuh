@@ -39,6 +39,9 @@
 // barrier shared with another warp).  A unit inside one run is finished by its
 // warp; the pieces of a cut unit meet in shared memory when its warps share a
 // CTA, and otherwise in the merge kernel, always in order of the keys.
+#include <mutex>
+#include <set>
+
 #include "kvq_attn_impl.cuh"
 #include "kvq_paged.cuh"
 
@@ -380,8 +383,14 @@ __device__ __forceinline__ void load_pairs(float (&s)[NG], float (&z)[NG], const
   attn::lds_words<NG * 4>(w, p);
 #pragma unroll
   for (int i = 0; i < NG; i++) {
-    s[i] = attn::dt_to_f<BF>((uint16_t)w[i]);
-    z[i] = attn::dt_to_f<BF>((uint16_t)(w[i] >> 16));
+    if constexpr (BF) {
+      s[i] = __uint_as_float(w[i] << 16);
+      z[i] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const __half2 h = *reinterpret_cast<const __half2*>(&w[i]);
+      s[i] = __low2float(h);
+      z[i] = __high2float(h);
+    }
   }
 }
 
@@ -677,7 +686,27 @@ __global__ void __launch_bounds__(Cfg<BITS, D, GS, NT, ST>::W * 32, 1)
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   Plan P;
-  if (ws.tpre) {
+  const int fixed = v.B * ((a.rep + NC - 1) / NC);  // column blocks of a decode
+  if (!v.cu && fixed <= 32) {
+    // few sequences: every warp makes the plan with its lanes and writes the
+    // same values, so no barrier stands before the first copy
+    long long* tpre = reinterpret_cast<long long*>(smem + C::O_PLAN);
+    P = Plan{nullptr, tpre, fixed};
+    int n = lane < fixed ? get_block<NC>(a, P, lane).nt : 0;
+    long long e = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, e, o);
+      if (lane >= o) e += y;
+    }
+    if (lane < fixed) tpre[lane + 1] = e;
+    if (lane == 0) tpre[0] = 0;
+    if (blockIdx.x == 0 && w == 0 && lane < v.B) {
+      int row0, rn, len;
+      checked_rows(v, lane, row0, rn, len, true);
+    }
+    __syncwarp();
+  } else if (ws.tpre) {
     P = Plan{ws.gpre, ws.tpre, *ws.ng};
     __syncthreads();
   } else {
@@ -689,8 +718,8 @@ __global__ void __launch_bounds__(Cfg<BITS, D, GS, NT, ST>::W * 32, 1)
   }
   const long long RT = P.tpre[P.NG] * v.Hkv;
   const long long all = (long long)gridDim.x * W, gw = (long long)blockIdx.x * W + w;
-  // at least two stages per warp: a shorter run costs more in merging
-  const long long act = max(1ll, min(all, RT / (2 * TPS)));
+  // at least one stage per warp
+  const long long act = max(1ll, min(all, RT / TPS));
   const long long t0 = gw < act ? gw * RT / act : RT, t1 = gw < act ? (gw + 1) * RT / act : RT;
 
   // column blocks that see no key: zero rows
@@ -715,25 +744,29 @@ __global__ void __launch_bounds__(Cfg<BITS, D, GS, NT, ST>::W * 32, 1)
     Block kc = get_block<NC>(a, P, gi);
     long long rel = t0 - P.tpre[gi] * v.Hkv;
     int hc = (int)(rel / kc.nt), ic = (int)(rel - (long long)hc * kc.nt);
-    int left = (int)(t1 - t0);  // tiles to consume
+    int left = (int)(t1 - t0);  // tiles to consume, this segment's included
 
     // The issue side runs ahead.  Lane i holds the source of tile ibase + i of
     // its unit and issues that tile's copy itself; the page numbers of the 32
     // tiles after those are already on their way.
     const int32_t* itable;
-    int insink, ilo, int_, gii = gi, ih = hc, ii = ic, ibase = ic, ileft = left;
-    int next_page = -1, my_j0 = -1;
-    const uint8_t* my_src = nullptr;
-    unsigned have = 0;
+    int insink, ilo, int_, gii = gi, ih = hc, ii = ic, ibase, iwin, iend, irest = left;
+    int next_page, my_j0, my_bytes;
+    const uint8_t* my_src;
+    int istage = 0;
     auto tile_at = [&](int i) { return i < insink ? i : ilo + i - insink; };
     auto fetch = [&](int i) { return i < int_ ? __ldg(itable + (tile_at(i) >> v.tiles_shift)) : -1; };
-    auto place = [&](int page) {  // lane's tile ibase + lane in `page`
+    auto place = [&](int page) {  // tiles ii.. of the unit, lane's in `page`
+      ibase = ii;
+      iwin = min(iend, ibase + 32);
       const int tt = tile_at(ibase + lane);
-      const bool in = ibase + lane < int_, ok = in && page >= 0 && page < v.num_pages;
+      const bool in = ibase + lane < iwin, ok = in && page >= 0 && page < v.num_pages;
       if (in && !ok) raise(v);
       my_src = tile_ptr(v, ok ? page : 0, ih, tt & ((1 << v.tiles_shift) - 1));
       my_j0 = ok ? tt << 4 : -1;
-      have = __ballot_sync(0xffffffffu, ok);
+      // bytes of the stage that starts with the lane's tile; -1: no such tile
+      const unsigned have = __ballot_sync(0xffffffffu, ok);
+      my_bytes = in ? __popc((have >> lane) & ((1 << TPS) - 1)) * C::TILE : -1;
       next_page = fetch(ibase + 32 + lane);
     };
     auto set_unit = [&](const Block& k) {
@@ -741,40 +774,35 @@ __global__ void __launch_bounds__(Cfg<BITS, D, GS, NT, ST>::W * 32, 1)
       insink = k.nsink;
       ilo = k.lo;
       int_ = k.nt;
+      iend = min(int_, ii + irest);
+      irest -= iend - ii;
+      place(fetch(ii + lane));
     };
     set_unit(kc);
-    place(fetch(ibase + lane));
-    int istage = 0, flying = 0;
     auto issue = [&]() {
-      if (ileft <= 0) return;
-      if (ii == int_) {  // next unit
-        if (++ih == v.Hkv) {
-          ih = 0;
-          do {
-            gii++;
-          } while (P.tpre[gii + 1] == P.tpre[gii]);
+      if (ii == iwin) {
+        if (ii < iend) {
+          place(next_page);
+        } else {
+          if (irest == 0) return;
+          if (++ih == v.Hkv) {
+            ih = 0;
+            do {
+              gii++;
+            } while (P.tpre[gii + 1] == P.tpre[gii]);
+          }
+          ii = 0;
           set_unit(get_block<NC>(a, P, gii));
         }
-        ii = ibase = 0;
-        place(fetch(lane));
-      } else if (ii - ibase == 32) {
-        ibase = ii;
-        place(next_page);
       }
-      const int n = min(min(TPS, int_ - ii), ileft), off = lane - (ii - ibase);
-      const unsigned got = (have >> (ii - ibase)) & ((1u << n) - 1u);
-      if ((unsigned)off < (unsigned)n) {
-        if (off == 0) {
-          if (got) attn::mbar_expect_tx(bars + istage, __popc(got) * C::TILE);
-          else attn::mbar_arrive(bars + istage);
-        }
+      const int off = lane - (ii - ibase);
+      if ((unsigned)off < (unsigned)TPS && my_bytes >= 0) {
+        if (off == 0) attn::mbar_expect_tx(bars + istage, my_bytes);
         meta[istage * TPS + off] = my_j0;
         if (my_j0 >= 0)
           attn::bulk_g2s(ring + istage * C::STAGE + off * C::TILE, my_src, C::TILE, bars + istage);
       }
-      ii += n;
-      ileft -= n;
-      flying++;
+      ii = min(ii + TPS, iwin);
       istage = istage + 1 == STAGES ? 0 : istage + 1;
     };
 #pragma unroll 1
@@ -786,38 +814,45 @@ __global__ void __launch_bounds__(Cfg<BITS, D, GS, NT, ST>::W * 32, 1)
     bool begun = ic == 0;  // this segment holds the unit's first tile
     int stage = 0;
     uint32_t phase = 0;
-    bool dead = false;
     while (left > 0) {
-      const int n = min(min(TPS, kc.nt - ic), left);
-      __syncwarp();
-      if (flying > 0 && !attn::mbar_wait(bars + stage, phase)) {
-        dead = true;  // no copy is issued any more; those in flight are waited for
-        if (lane == 0) raise(v);
-      }
-      flying--;
-      const uint8_t* st = ring + stage * C::STAGE;
-      bool full = n == TPS;
-      int j0[TPS];
+      // list indices [fa, fb): tiles that every column sees whole
+      const int e = min(kc.nt, ic + left);
+      const int fa = a.window == 0 ? 0
+                                   : kc.nsink + max(0, ((kc.pmax - a.window + 16) >> 4) - kc.lo);
+      const int fb = min(e, kc.nsink + ((kc.pmin - 15) >> 4) - kc.lo + 1);
+      left -= e - ic;
+#pragma unroll 1
+      while (ic < e) {
+        __syncwarp();
+        if (!attn::mbar_wait(bars + stage, phase)) {
+          // give up: wait (bounded) for the copies still in flight, then leave
+          if (lane == 0) raise(v);
+          for (int s = 1; s < STAGES; s++) attn::mbar_wait(bars + (stage + s) % STAGES, (stage + s) / STAGES ^ phase);
+          left = 0;
+          break;
+        }
+        const uint8_t* st = ring + stage * C::STAGE;
+        int j0[TPS], bad = 0;
 #pragma unroll
-      for (int i = 0; i < TPS; i++) {
-        j0[i] = i < n ? meta[stage * TPS + i] : -1;
-        full = full && j0[i] >= 0 && j0[i] + 15 <= kc.pmin &&
-               (a.window == 0 || j0[i] > kc.pmax - a.window || j0[i] + 15 < a.sinks);
+        for (int i = 0; i < TPS; i++) {
+          j0[i] = meta[stage * TPS + i];
+          bad |= j0[i];
+        }
+        if (ic >= fa && ic + TPS <= fb && bad >= 0) {
+          process<BITS, D, GS, NT, ST, BF, TPS, false>(S, st, j0, a.window, a.sinks, g, t);
+        } else {
+          if (TPS == 2 && ic + 1 == e) j0[TPS - 1] = -1;
+          process<BITS, D, GS, NT, ST, BF, TPS, true>(S, st, j0, a.window, a.sinks, g, t);
+        }
+        __syncwarp();
+        issue();
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+        ic += TPS;
       }
-      if (full) {
-        process<BITS, D, GS, NT, ST, BF, TPS, false>(S, st, j0, a.window, a.sinks, g, t);
-      } else {
-        process<BITS, D, GS, NT, ST, BF, TPS, true>(S, st, j0, a.window, a.sinks, g, t);
-      }
-      __syncwarp();
-      if (!dead) issue();
-      if (++stage == STAGES) {
-        stage = 0;
-        phase ^= 1;
-      }
-      ic += n;
-      left -= n;
-      if (ic < kc.nt && left > 0) continue;
+      ic = e;
 
       // the segment ends: the unit is done, or the warp's run is
       close<BITS, D, GS, NT, ST, BF>(S);
@@ -1030,6 +1065,19 @@ __global__ void __launch_bounds__(1024) plan_kernel(const AttnArgs a, const Work
   if (threadIdx.x == 0) *ws.ng = NG;
 }
 
+// The merge keeps the column kernel's split of the SM's memory, so that it can
+// become resident without waiting for the SM to empty.
+inline int32_t kernel_carveout(const void* kern, int dev) {
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> done;
+  std::lock_guard<std::mutex> lk(mu);
+  if (done.count({kern, dev})) return KVQ_OK;
+  KVQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                    cudaSharedmemCarveoutMaxShared));
+  done.insert({kern, dev});
+  return KVQ_OK;
+}
+
 template <int BITS, int D, int GS, int NT, int ST, bool BF>
 int32_t launch_cols_one(const AttnArgs& a, const Work& ws, int ctas, int dev, cudaStream_t st) {
   using C = Cfg<BITS, D, GS, NT, ST>;
@@ -1038,8 +1086,10 @@ int32_t launch_cols_one(const AttnArgs& a, const Work& ws, int ctas, int dev, cu
   if (rc) return rc;
   if (ws.tpre) KVQ_CUDA_TRY(launch_pdl(plan_kernel<C::NC>, dim3(1), dim3(1024), 0, st, a, ws));
   KVQ_CUDA_TRY(launch_pdl(kern, dim3((unsigned)ctas), dim3(C::W * 32), C::SMEM, st, a, ws));
-  KVQ_CUDA_TRY(launch_pdl(cols_merge_kernel<BITS, D, GS, NT, ST, BF>, dim3((unsigned)ctas, C::FR),
-                          dim3(kMergeWarps * 32), 0, st, a, ws));
+  auto merge = cols_merge_kernel<BITS, D, GS, NT, ST, BF>;
+  const int32_t rm = kernel_carveout(reinterpret_cast<const void*>(merge), dev);
+  if (rm) return rm;
+  KVQ_CUDA_TRY(launch_pdl(merge, dim3((unsigned)ctas, C::FR), dim3(kMergeWarps * 32), 0, st, a, ws));
   return KVQ_OK;
 }
 

@@ -20,6 +20,7 @@ from .cache import dtype_code
 
 TILE_ROWS = 16
 _I64x2 = ctypes.c_int64 * 2
+_byref = ctypes.byref
 
 
 @dataclass
@@ -78,6 +79,8 @@ class PagedQuantizedKVCache:
         self.pool = pool
         self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._c.pool, self._c.status = pool.data_ptr(), self._status.data_ptr()
+        self._index, self._ref = index, _byref(self._c)
+        self._ws_bytes = {}
 
     @staticmethod
     def pool_shape(num_pages: int, page_size: int, kv_heads: int, head_dim: int,
@@ -110,37 +113,44 @@ class PagedQuantizedKVCache:
     # ------------------------------------------------------------- a step --
 
     def _batch(self, rows: int, page_table, seq_lens, cu_rows) -> _lib.PagedBatch:
-        dev = self.device
-        B = seq_lens.shape[0]
-        if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B or \
-                (page_table.shape[1] > 1 and page_table.stride(1) != 1) or page_table.device != dev:
+        i32, dev = torch.int32, self._index
+        B, pages = seq_lens.shape[0], page_table.shape
+        if page_table.dtype is not i32 or len(pages) != 2 or pages[0] != B or \
+                page_table.get_device() != dev or (pages[1] > 1 and page_table.stride(1) != 1):
             raise ValueError("page_table must be int32 [batch, max_pages] with contiguous rows on "
                              "the cache's device")
-        if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or seq_lens.device != dev or \
+        if seq_lens.dtype is not i32 or seq_lens.dim() != 1 or seq_lens.get_device() != dev or \
                 not seq_lens.is_contiguous():
             raise ValueError("seq_lens must be contiguous int32 [batch] on the cache's device")
-        if cu_rows is not None and (cu_rows.dtype != torch.int32 or cu_rows.dim() != 1 or
-                                    cu_rows.shape[0] != B + 1 or cu_rows.device != dev or
-                                    not cu_rows.is_contiguous()):
-            raise ValueError("cu_rows must be contiguous int32 [batch + 1] on the cache's device")
-        return _lib.PagedBatch(page_table.data_ptr(), max(page_table.stride(0), page_table.shape[1]),
-                               seq_lens.data_ptr(),
-                               cu_rows.data_ptr() if cu_rows is not None else None, B,
-                               page_table.shape[1], rows)
+        cu = None
+        if cu_rows is not None:
+            if cu_rows.dtype is not i32 or cu_rows.dim() != 1 or cu_rows.shape[0] != B + 1 or \
+                    cu_rows.get_device() != dev or not cu_rows.is_contiguous():
+                raise ValueError("cu_rows must be contiguous int32 [batch + 1] on the cache's device")
+            cu = cu_rows.data_ptr()
+        return _lib.PagedBatch(page_table.data_ptr(), max(page_table.stride(0), pages[1]),
+                               seq_lens.data_ptr(), cu, B, pages[1], rows)
 
     def _rows(self, x: torch.Tensor, name: str, heads: int | None = None):
-        """Check token rows [rows, heads, head_dim]; returns (rows, heads, strides)."""
-        if x.dim() != 3 or x.shape[2] != self.head_dim or (heads is not None and x.shape[1] != heads):
+        """Check token rows [rows, heads, head_dim]; returns (shape, strides)."""
+        shape = x.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
             raise ValueError(f"{name} must be [rows, {heads or 'heads'}, {self.head_dim}]")
-        if x.dtype != self.dtype or x.device != self.device:
+        if x.dtype is not self.dtype or x.get_device() != self._index:
             raise ValueError(f"{name} must be {self.dtype} on {self.device}")
         s = x.stride()
         if s[2] != 1:
             raise ValueError(f"{name}: the last dimension must be contiguous")
-        return x.shape[0], x.shape[1], _I64x2(s[0], s[1])
+        return shape, _I64x2(s[0], s[1])
+
+    def _like(self, x: torch.Tensor, shape, name: str):
+        if x.shape != shape or x.dtype is not self.dtype or x.get_device() != self._index or \
+                not x.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous tensor like q")
 
     def _stream(self, stream):
-        return torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream
+        # the raw handle of torch's current stream (or the caller's)
+        return torch._C._cuda_getCurrentRawStream(self._index) if stream is None else stream
 
     def append(self, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
                seq_lens: torch.Tensor, cu_rows: torch.Tensor | None = None,
@@ -153,48 +163,58 @@ class PagedQuantizedKVCache:
         contiguous q in place), which is returned.  Padding rows (from
         cu_rows[batch] on) are not touched: a fresh q_out holds anything
         there."""
-        rows, _, ks = self._rows(k, "k", self.kv_heads)
-        vrows, _, vs = self._rows(v, "v", self.kv_heads)
-        if vrows != rows:
+        shape, ks = self._rows(k, "k", self.kv_heads)
+        vshape, vs = self._rows(v, "v", self.kv_heads)
+        rows = shape[0]
+        if vshape[0] != rows:
             raise ValueError("k and v must have the same rows")
         batch = self._batch(rows, page_table, seq_lens, cu_rows)
-        qh, qs, qp = 0, None, None
+        qh, qs, qp, op = 0, None, None, None
         if q is not None:
-            qrows, qh, qs = self._rows(q, "q")
-            if qrows != rows:
+            qshape, qs = self._rows(q, "q")
+            if qshape[0] != rows:
                 raise ValueError("q and k must have the same rows")
+            qh = qshape[1]
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != q.device or \
-                    not q_out.is_contiguous():
-                raise ValueError("q_out must be a contiguous tensor like q")
-            qp = q.data_ptr()
+                q_out = torch.empty(qshape, dtype=q.dtype, device=q.device)
+            else:
+                self._like(q_out, qshape, "q_out")
+            qp, op = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out needs q")
-        r = ctypes.byref(rope._struct(self.device)) if rope is not None else None
-        check(lib().kvq_paged_append(ctypes.byref(self._c), ctypes.byref(batch), k.data_ptr(),
-                                     v.data_ptr(), ks, vs, r, qp, qh, qs,
-                                     q_out.data_ptr() if q_out is not None else None,
-                                     self._stream(stream)))
+        r = _byref(rope._struct(self.device)) if rope is not None else None
+        rc = lib().kvq_paged_append(self._ref, _byref(batch), k.data_ptr(), v.data_ptr(), ks, vs, r,
+                                    qp, qh, qs, op, self._stream(stream))
+        if rc:
+            check(rc)
         return q_out
 
-    def _sdpa(self, decode, q, page_table, seq_lens, cu_rows, scale, window, sinks, out,
-              workspace, stream):
-        rows, qh, qs = self._rows(q, "q")
-        batch = self._batch(rows, page_table, seq_lens, cu_rows)
+    def _sdpa(self, fn, q, page_table, seq_lens, cu_rows, scale, window, sinks, out, workspace,
+              stream):
+        shape, qs = self._rows(q, "q")
+        batch = self._batch(shape[0], page_table, seq_lens, cu_rows)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or \
-                not out.is_contiguous():
-            raise ValueError("out must be a contiguous tensor like q")
+            out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        else:
+            self._like(out, shape, "out")
         ws, wsb = None, 0
         if workspace is not None:
-            if workspace.device != self.device or not workspace.is_contiguous():
+            if workspace.get_device() != self._index or not workspace.is_contiguous():
                 raise ValueError("workspace must be a contiguous tensor on the cache's device")
             ws, wsb = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        fn = lib().kvq_paged_sdpa_decode if decode else lib().kvq_paged_sdpa_prefill
-        check(fn(ctypes.byref(self._c), ctypes.byref(batch), q.data_ptr(), qh, qs, scale, window,
-                 sinks, out.data_ptr(), ws, wsb, self._stream(stream)))
+        elif stream is None:
+            # torch's allocator orders it on the current stream and gives a
+            # captured graph memory of its own; the size goes by the shapes
+            key = (cu_rows is None, shape[0], batch.batch, shape[1])
+            wsb = self._ws_bytes.get(key)
+            if wsb is None:
+                wsb = self._ws_bytes[key] = self._workspace(batch, shape[1], cu_rows is None)
+            workspace = torch.empty(wsb, dtype=torch.uint8, device=self.device)
+            ws = workspace.data_ptr()
+        rc = fn(self._ref, _byref(batch), q.data_ptr(), shape[1], qs, scale, window, sinks,
+                out.data_ptr(), ws, wsb, self._stream(stream))
+        if rc:
+            check(rc)
         return out
 
     def sdpa_decode(self, q: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -205,8 +225,8 @@ class PagedQuantizedKVCache:
         head_dim], at the sequences' last positions (kvq_paged_sdpa_decode).
         window > 0: the last `window` keys and the first `sinks` ones.
         workspace None: the call's own, safe with calls on other streams."""
-        return self._sdpa(True, q, page_table, seq_lens, None, scale, window, sinks, out,
-                          workspace, stream)
+        return self._sdpa(lib().kvq_paged_sdpa_decode, q, page_table, seq_lens, None, scale, window,
+                          sinks, out, workspace, stream)
 
     def sdpa_prefill(self, q: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
                      cu_rows: torch.Tensor, scale: float, window: int = 0, sinks: int = 0,
@@ -216,17 +236,20 @@ class PagedQuantizedKVCache:
         sequence b's rows are cu_rows[b]..cu_rows[b + 1] and end at its last
         position (kvq_paged_sdpa_prefill).  Padding rows are not touched: a
         fresh `out` holds anything there."""
-        return self._sdpa(False, q, page_table, seq_lens, cu_rows, scale, window, sinks, out,
-                          workspace, stream)
+        return self._sdpa(lib().kvq_paged_sdpa_prefill, q, page_table, seq_lens, cu_rows, scale,
+                          window, sinks, out, workspace, stream)
 
     def workspace_bytes(self, rows: int, q_heads: int, page_table: torch.Tensor,
                         seq_lens: torch.Tensor, cu_rows: torch.Tensor | None = None) -> int:
         """Bytes a caller's workspace needs for sdpa_decode (cu_rows None) or
         sdpa_prefill of these shapes."""
-        batch = self._batch(rows, page_table, seq_lens, cu_rows)
+        return self._workspace(self._batch(rows, page_table, seq_lens, cu_rows), q_heads,
+                               cu_rows is None)
+
+    def _workspace(self, batch, q_heads: int, decode: bool) -> int:
         n = ctypes.c_size_t()
-        check(lib().kvq_paged_sdpa_workspace(ctypes.byref(self._c), ctypes.byref(batch), q_heads,
-                                             0 if cu_rows is not None else 1, ctypes.byref(n)))
+        check(lib().kvq_paged_sdpa_workspace(self._ref, _byref(batch), q_heads, int(decode),
+                                             _byref(n)))
         return n.value
 
     def check(self, stream=None):
