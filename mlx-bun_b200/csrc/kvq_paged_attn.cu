@@ -2,7 +2,7 @@
 // workspace and its launches.
 #include <algorithm>
 
-#include "kvq_paged_cols.cuh"
+#include "kvq_paged_chunk.cuh"
 
 namespace kvq {
 namespace paged {
@@ -16,20 +16,34 @@ int32_t launch_cols<8, false>(const AttnArgs&, const Work&, int, int, int, cudaS
 template <>
 int32_t launch_cols<8, true>(const AttnArgs&, const Work&, int, int, int, cudaStream_t);
 
+template <>
+int32_t launch_chunk<4, false>(const AttnArgs&, const Work&, int, int, cudaStream_t);
+template <>
+int32_t launch_chunk<4, true>(const AttnArgs&, const Work&, int, int, cudaStream_t);
+template <>
+int32_t launch_chunk<8, false>(const AttnArgs&, const Work&, int, int, cudaStream_t);
+template <>
+int32_t launch_chunk<8, true>(const AttnArgs&, const Work&, int, int, cudaStream_t);
+
 namespace {
+
+// Query rows (times heads of a group) per sequence above which a call goes to
+// the chunk kernel.
+constexpr long long kChunkCols = 64;
 
 size_t up16(size_t x) { return (x + 15) / 16 * 16; }
 
-// The column kernel's launch: columns per block, CTAs and workspace layout.
-struct ColsLaunch {
+// The launch: kernel, columns (query rows) per block, CTAs, workspace layout.
+struct Launch {
+  bool chunk;
   int NC, ctas;
   long long max_blocks;
   bool big;  // the plan does not fit in shared memory
   size_t o_meta, o_gpre, o_tpre, o_ng, bytes;
 };
 
-ColsLaunch cols_launch(const AttnArgs& a) {
-  ColsLaunch c{};
+Launch plan_launch(const AttnArgs& a) {
+  Launch c{};
   const View& v = a.v;
   int dev = 0;
   cudaGetDevice(&dev);
@@ -37,11 +51,13 @@ ColsLaunch cols_launch(const AttnArgs& a) {
   // columns per block: 16 where a sequence has more than 8 (K and V are read
   // once for all; D 256 has no registers for them), 4 where it has no more
   const long long cols = (long long)v.rows * a.rep;
-  c.NC = cols > 8ll * v.B ? (v.D < 256 ? 16 : 8) : (cols > 4ll * v.B ? 8 : 4);
+  c.chunk = v.cu && cols > kChunkCols * v.B;
+  c.NC = c.chunk ? (v.D == 256 ? 128 : 256) : cols > 8ll * v.B ? (v.D < 256 ? 16 : 8) : (cols > 4ll * v.B ? 8 : 4);
   const int NC = c.NC, NT = NC > 8 ? 2 : 1;
   c.max_blocks = v.cu ? cols / NC + v.B : (long long)v.B * ((a.rep + NC - 1) / NC);
   c.big = v.B > kPlanMax || c.max_blocks > kPlanMax;
-  const size_t piece = (size_t)(16 * NT + v.D / 16 * NT * 128) * 4;
+  const size_t piece = c.chunk ? (size_t)NC * (v.D + 2) * 4
+                               : (size_t)(16 * NT + v.D / 16 * NT * 128) * 4;
   c.o_meta = 2 * (size_t)c.ctas * piece;
   c.o_gpre = c.o_meta + (size_t)c.ctas * 16;
   c.bytes = c.o_gpre;
@@ -59,10 +75,10 @@ bool vec_ok(const AttnArgs& a) {
 
 }  // namespace
 
-size_t paged_attn_workspace(const AttnArgs& a) { return cols_launch(a).bytes; }
+size_t paged_attn_workspace(const AttnArgs& a) { return plan_launch(a).bytes; }
 
 int32_t launch_paged_attn(const AttnArgs& a, void* ws, size_t, cudaStream_t st) {
-  const ColsLaunch c = cols_launch(a);
+  const Launch c = plan_launch(a);
   if (c.max_blocks * a.v.Hkv > 0x7fffffff) return fail(KVQ_ERR_ARG, "paged: too many rows * heads in one call");
   uint8_t* p = static_cast<uint8_t*>(ws);
   Work w{};
@@ -77,6 +93,13 @@ int32_t launch_paged_attn(const AttnArgs& a, void* ws, size_t, cudaStream_t st) 
   w.vec = vec_ok(a);
   int dev = 0;
   KVQ_CUDA_TRY(cudaGetDevice(&dev));
+  if (c.chunk) {
+    if (a.v.bits == 4)
+      return a.bf16 ? launch_chunk<4, true>(a, w, c.ctas, dev, st)
+                    : launch_chunk<4, false>(a, w, c.ctas, dev, st);
+    return a.bf16 ? launch_chunk<8, true>(a, w, c.ctas, dev, st)
+                  : launch_chunk<8, false>(a, w, c.ctas, dev, st);
+  }
   if (a.v.bits == 4)
     return a.bf16 ? launch_cols<4, true>(a, w, c.NC, c.ctas, dev, st)
                   : launch_cols<4, false>(a, w, c.NC, c.ctas, dev, st);

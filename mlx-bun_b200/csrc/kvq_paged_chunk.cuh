@@ -1,0 +1,686 @@
+#pragma once
+// kvq_paged_chunk.cuh — attention of many query rows per sequence over the
+// pages (prompt chunks) on the tcgen05 tensor cores.
+//
+// A unit is one (sequence, kv head) and MR query rows (row c is token c / rep,
+// head c % rep: every query head of the group shares the tile's K and V).  Its
+// 128-key tiles are dequantized once, to the dtype, into 128-byte-swizzled
+// shared tiles and serve all MR rows: S = Q K^T into TMEM, softmax from TMEM
+// to P in the same columns, O += P V with A from TMEM.
+//   * D 64 / 128: MR 256, two row tiles of 128 (TMEM lanes) in turn: the tensor
+//     core works on one while the softmax warps have the other.
+//   * D 256: MR 128 (its O takes 256 TMEM columns), two S buffers instead.
+// Warps: 4 per row tile for the softmax (a thread owns a row, no shuffles), 4
+// that dequantize K, 4 for V (a thread owns a key row and loads the next
+// tile's codes before it waits for its buffer), 1 that issues the MMAs.
+// All hand-offs are mbarriers with bounded waits.
+//
+// Roundings: K, V (as a dense cache of the dtype holds them) and the
+// probabilities go through the tensor core in the dtype; logits, statistics
+// and O are f32.  O is rescaled only when a row's maximum has grown by more
+// than 2^8 since the last time (p stays below 256, its sum in f32).
+//
+// Bound: per 128 keys and 256 rows at D 128 the tensor core needs 2048 clocks
+// (8192 dense flops a clock) and so do the exponentials (16 a clock per SM).
+//
+// Work split: the tiles of all units laid end to end, one equal run per SM;
+// the pieces of a cut unit (m, l, O in f32) meet in the merge kernel in order.
+#include "kvq_paged_cols.cuh"
+#include "kvq_tc.cuh"
+
+namespace kvq {
+namespace paged {
+
+template <int BITS, int D, int GS>
+struct Chunk {
+  static constexpr int QT = D == 256 ? 1 : 2;   // row tiles of 128
+  static constexpr int MR = 128 * QT;
+  static constexpr int KT = 128;                // keys per tile
+  static constexpr int KB = D == 256 ? 1 : 2;   // K (and V) buffers
+  static constexpr int PANEL = 128 * 128;       // bytes: 128 rows of 64 elements
+  static constexpr int TILE = D / 64 * PANEL;   // bytes of a Q, K or V tile
+  static constexpr int CRB = D * BITS / 8;
+  static constexpr int PRB = D / GS * 4;
+  static constexpr int HALF = kTileRows * (CRB + PRB);
+  static constexpr int O_Q = 0;
+  static constexpr int O_K = QT * TILE;
+  static constexpr int O_V = O_K + KB * TILE;
+  static constexpr int O_PLAN = O_V + KB * TILE;
+  static constexpr int O_TMP = (O_PLAN + (kPlanMax + 1) * 12 + 4 + 15) / 16 * 16;
+  static constexpr int O_BAR = O_TMP + 34 * 8;
+  static constexpr int O_MISC = O_BAR + 24 * 8;  // TMEM address, bad tiles [4][4]
+  static constexpr int SMEM = O_MISC + 64 + 1024;  // + alignment of the swizzled tiles
+  static constexpr int kSoftWarps = 4 * QT;
+  static constexpr int kThreads = (kSoftWarps + 9) * 32;
+  static constexpr int TM_O = 256;              // TMEM columns: S at 0 and 128, O from 256
+  static constexpr int PIECE = MR * (D + 2);    // floats: m [MR], l [MR], O [D / 4][MR][4]
+  static_assert(SMEM <= 232448, "shared memory");
+};
+
+struct ChunkBars {
+  uint64_t q_full[2], s_full[2], p_full[2], o_done[2];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+};
+
+// The segments (runs of tiles inside one unit) of a CTA, walked by each role.
+template <int BITS, int D, int GS>
+struct Walk {
+  using C = Chunk<BITS, D, GS>;
+  Plan P;
+  int gi, h, i0, i1;   // tiles [i0, i1) of the unit's list
+  long long left;
+  Block k;
+
+  __device__ __forceinline__ void start(const AttnArgs& a, const Plan& plan, long long t0, long long t1) {
+    P = plan;
+    left = t1 - t0;
+    if (left <= 0) return;
+    const int Hkv = a.v.Hkv;
+    int x = 0, y = P.NG;
+    while (y - x > 1) {
+      const int mid = (x + y) >> 1;
+      if (P.tpre[mid] * Hkv <= t0) x = mid;
+      else y = mid;
+    }
+    gi = x;
+    k = get_block<C::MR, 7>(a, P, gi);
+    const long long rel = t0 - P.tpre[gi] * Hkv;
+    h = (int)(rel / k.nt);
+    i0 = (int)(rel - (long long)h * k.nt);
+    i1 = (int)min((long long)k.nt, i0 + left);
+  }
+  __device__ __forceinline__ bool valid() const { return left > 0; }
+  __device__ __forceinline__ void next(const AttnArgs& a) {
+    left -= i1 - i0;
+    if (left <= 0) return;
+    if (++h == a.v.Hkv) {
+      h = 0;
+      do {
+        gi++;
+      } while (P.tpre[gi + 1] == P.tpre[gi]);
+      k = get_block<C::MR, 7>(a, P, gi);
+    }
+    i0 = 0;
+    i1 = (int)min((long long)k.nt, left);
+  }
+};
+
+// 8 codes to 8 dtype values code * s + z, one rounding.  4-bit words give them
+// in the order 0 4 1 5 2 6 3 7 (Q is laid out alike, and O's columns are put
+// back when they are written), 8-bit words in their own.
+template <int BITS, bool BF>
+struct Dequant {
+  uint32_t s2, z2;  // scale and bias, twice
+  float sf, zf;
+  __device__ __forceinline__ explicit Dequant(uint32_t pair) {
+    s2 = prmt(pair, 0u, 0x1010u);
+    z2 = prmt(pair, 0u, 0x3232u);
+    sf = attn::dt_to_f<BF>((uint16_t)pair);
+    zf = attn::dt_to_f<BF>((uint16_t)(pair >> 16));
+  }
+  static __device__ __forceinline__ uint32_t fma_h(uint32_t c, uint32_t s, uint32_t z) {
+    const __half2 r = __hfma2(*reinterpret_cast<__half2*>(&c), *reinterpret_cast<__half2*>(&s),
+                              *reinterpret_cast<__half2*>(&z));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ uint32_t fma_b(uint32_t c, uint32_t s, uint32_t z) {
+    const __nv_bfloat162 r =
+        __hfma2(*reinterpret_cast<__nv_bfloat162*>(&c), *reinterpret_cast<__nv_bfloat162*>(&s),
+                *reinterpret_cast<__nv_bfloat162*>(&z));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  // w: 1 word of 4-bit or 2 words of 8-bit codes
+  __device__ __forceinline__ uint4 eight(const uint32_t* w) const {
+    uint32_t r[4];
+    if constexpr (BITS == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if constexpr (BF) {
+          // 128 + c, minus 128
+          const uint32_t x = ((w[0] >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+          r[i] = fma_b(fma_b(x, 0x3f803f80u, 0xc300c300u), s2, z2);
+        } else {
+          // 1024 + c minus 1024; odd nibbles (1024 + 16 c) / 16 - 64
+          const uint32_t y = i >= 2 ? w[0] >> 8 : w[0];
+          const uint32_t x = (y & ((i & 1) ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;
+          r[i] = fma_h((i & 1) ? fma_h(x, 0x2c002c00u, 0xd400d400u) : fma_h(x, 0x3c003c00u, 0xe400e400u),
+                       s2, z2);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint32_t u = w[i >> 1];
+        if constexpr (BF) {
+          // codes up to 255 have no bf16 form with a free offset: f32, rounded once
+          const float a = __uint_as_float(prmt(u, 0x4b000000u, (i & 1) ? 0x7442u : 0x7440u)) - 8388608.0f;
+          const float b = __uint_as_float(prmt(u, 0x4b000000u, (i & 1) ? 0x7443u : 0x7441u)) - 8388608.0f;
+          const __nv_bfloat162 t = __floats2bfloat162_rn(fmaf(a, sf, zf), fmaf(b, sf, zf));
+          r[i] = *reinterpret_cast<const uint32_t*>(&t);
+        } else {
+          const uint32_t x = prmt(u, 0x64646464u, (i & 1) ? 0x4342u : 0x4140u);
+          r[i] = fma_h(fma_h(x, 0x3c003c00u, 0xe400e400u), s2, z2);
+        }
+      }
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+  }
+};
+
+// position of list element i of a 4-bit word's eight values
+__device__ __forceinline__ constexpr int nib_pos(int i) { return (i >> 1) + (i & 1) * 4; }
+
+__device__ __forceinline__ uint32_t idesc_for(bool bf, int M, int N, int b_mn_major) {
+  return attn::tc::idesc_f16(M, N, b_mn_major) | (bf ? (1u << 7) | (1u << 10) : 0u);
+}
+// MN-major tile of several 64-element panels, PANEL bytes apart
+__device__ __forceinline__ uint64_t desc_panels(uint32_t saddr, uint32_t panel) {
+  return (attn::tc::desc_sw128(saddr) & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(panel >> 4) << 16);
+}
+
+template <int BITS, int D, int GS, bool BF>
+__global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
+    chunk_kernel(const AttnArgs a, const Work ws) {
+  using C = Chunk<BITS, D, GS>;
+  using namespace attn::tc;
+  constexpr int QT = C::QT, KB = C::KB, NG = D / GS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = smem_raw + ((1024 - (attn::smem_u32(smem_raw) & 1023)) & 1023);
+  const View& v = a.v;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  ChunkBars& bar = *reinterpret_cast<ChunkBars*>(sm + C::O_BAR);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(sm + C::O_MISC);
+  volatile uint8_t* s_bad = sm + C::O_MISC + 16;  // [4 tiles in flight][4 warps]
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) {
+    for (int i = 0; i < 2; i++) {
+      attn::mbar_init(&bar.q_full[i], 128);
+      attn::mbar_init(&bar.s_full[i], 1);
+      attn::mbar_init(&bar.p_full[i], 128);
+      attn::mbar_init(&bar.o_done[i], 1);
+      attn::mbar_init(&bar.k_full[i], 128);
+      attn::mbar_init(&bar.k_empty[i], 1);
+      attn::mbar_init(&bar.v_full[i], 128);
+      attn::mbar_init(&bar.v_empty[i], 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == C::kSoftWarps + 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     attn::smem_u32(s_tmem)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  Plan P;
+  if (ws.tpre) {
+    P = Plan{ws.gpre, ws.tpre, *ws.ng};
+  } else {
+    long long* tpre = reinterpret_cast<long long*>(sm + C::O_PLAN);
+    int* gpre = reinterpret_cast<int*>(tpre + kPlanMax + 1);
+    const int NG_ = build_plan<C::MR, 7>(a, gpre, tpre, ws.max_blocks,
+                                         reinterpret_cast<long long*>(sm + C::O_TMP), blockIdx.x == 0);
+    P = Plan{gpre, tpre, NG_};
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = *s_tmem;
+  const long long RT = P.tpre[P.NG] * v.Hkv;
+  const long long act = max(1ll, min((long long)gridDim.x, RT / 2));
+  const long long c = blockIdx.x;
+  const long long t0 = c < act ? c * RT / act : RT, t1 = c < act ? (c + 1) * RT / act : RT;
+  Walk<BITS, D, GS> wk;
+  wk.start(a, P, t0, t1);
+  // Bounded; a role that gives up leaves its loop, and the others' waits run
+  // out in turn.  The warp-wide form keeps the warp together.
+  auto wait = [&](uint64_t* b, int parity) -> bool {
+    if (attn::mbar_wait(b, (uint32_t)parity)) return true;
+    raise(v);
+    return false;
+  };
+  auto wait_all = [&](uint64_t* b, int parity) -> bool {
+    return __all_sync(0xffffffffu, wait(b, parity));
+  };
+  int slot1 = -1, slot0 = 0;  // this CTA's pieces (softmax threads)
+  Block slot_block{};
+
+  if (warp < C::kSoftWarps) {
+    // ------------------------------------------------ softmax: one row a thread
+    const int q = warp >> 2, r = (warp & 3) * 32 + lane;  // row tile, row in it
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const float c2 = fabsf(a.scale) * attn::kLog2e;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+    int tc = 0;  // tiles so far
+    bool ok = true;
+    for (int u = 0; wk.valid() && ok; wk.next(a), u++) {
+      const Block& k = wk.k;
+      const int row = q * 128 + r;
+      const bool live = row < k.cols;
+      const int col = k.col0 + (live ? row : 0), tok = col / a.rep;
+      const int64_t trow = k.row0 + tok;
+      const int head = wk.h * a.rep + (col - tok * a.rep);
+      const int p = live ? k.p0 + tok : -1;
+      {
+        const uint16_t* src = a.q + trow * a.q_row + (int64_t)head * a.q_head;
+        uint8_t* dst = sm + C::O_Q + q * C::TILE;
+#pragma unroll 4
+        for (int e = 0; e < D / 8; e++) {
+          uint16_t x[8];
+          if (ws.vec) {
+            const uint4 y = *reinterpret_cast<const uint4*>(src + e * 8);
+            const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = src[e * 8 + i];
+          }
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t lo = x[BITS == 4 ? nib_pos(2 * i) : 2 * i];
+            const uint32_t hi = x[BITS == 4 ? nib_pos(2 * i + 1) : 2 * i + 1];
+            w[i] = live ? (lo | (hi << 16)) ^ flip : 0u;
+          }
+          *reinterpret_cast<uint4*>(dst + (e >> 3) * C::PANEL + sw128(r, (e & 7) * 8)) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        attn::mbar_arrive(&bar.q_full[q]);
+      }
+      float m = kNeg, l = 0.0f;
+      for (int i = wk.i0; i < wk.i1; i++, tc++) {
+        const int sb = QT == 2 ? q : tc & 1;
+        const uint32_t tS = tm + lanes + sb * 128;
+        if (!wait_all(&bar.s_full[sb], QT == 2 ? tc & 1 : (tc >> 1) & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int kb = tile_of(k, i) << 7;
+        const uint32_t bad4 = *reinterpret_cast<volatile uint32_t*>(const_cast<uint8_t*>(s_bad) + (tc & 3) * 4);
+        const bool full = kb + 127 <= k.pmin && bad4 == 0 &&
+                          (a.window == 0 || kb > k.pmax - a.window || kb + 127 < a.sinks);
+        uint32_t vis[4];
+        if (!full) {
+          // bits of the tile's keys that this row sees
+#pragma unroll
+          for (int w = 0; w < 4; w++) {
+            const int j0 = kb + 32 * w;
+            auto upto = [](int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); };
+            uint32_t x = upto(p + 1 - j0);
+            if (a.window > 0) x &= ~upto(p - a.window + 1 - j0) | upto(a.sinks - j0);
+            const uint32_t b2 = (bad4 >> (8 * w)) & 3u;  // two 16-key tiles without a page
+            x &= ~(((b2 & 1u) ? 0x0000ffffu : 0u) | ((b2 & 2u) ? 0xffff0000u : 0u));
+            vis[w] = x;
+          }
+        }
+        float mx = kNeg;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          uint32_t s[32];
+          tmem_ld32(tS + 32 * w, s);
+          tmem_wait_ld();
+          if (full) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2)
+              mx = fmaxf(mx, fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+              if ((vis[w] >> e) & 1u) mx = fmaxf(mx, __uint_as_float(s[e]));
+          }
+        }
+        mx = mx > 0.5f * kNeg ? mx * c2 : kNeg;
+        const bool grow = mx > m + 8.0f;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float mn = fmaxf(m, mx), f = ex2(m - mn);
+          m = mn;
+          l *= f;
+          if (i > wk.i0) {
+            // every earlier product of this unit must have landed in O
+            if (!wait_all(&bar.o_done[QT == 2 ? q : 0], (tc - 1) & 1)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll 1
+            for (int d = 0; d < D; d += 32) {
+              uint32_t o[32];
+              const uint32_t tO = tm + lanes + C::TM_O + q * D + d;
+              tmem_ld32(tO, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32(tO, o);
+            }
+            tmem_wait_st();
+          }
+        }
+        const float2 cc = make_float2(c2, c2), mm = make_float2(-m, -m);
+        float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          uint32_t s[32], pk[16];
+          tmem_ld32(tS + 32 * w, s);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), cc, mm);
+            float2 y = make_float2(ex2(x.x), ex2(x.y));
+            if (!full) {
+              if (!((vis[w] >> e) & 1u)) y.x = 0.0f;
+              if (!((vis[w] >> (e + 1)) & 1u)) y.y = 0.0f;
+            }
+            sum = __fadd2_rn(sum, y);
+            if constexpr (BF) {
+              const __nv_bfloat162 t = __floats2bfloat162_rn(y.x, y.y);
+              pk[e / 2] = *reinterpret_cast<const uint32_t*>(&t);
+            } else {
+              pk[e / 2] = pack_h2(y.x, y.y);
+            }
+          }
+          // columns 16 w.. of P lie over columns of S that are read already
+          tmem_st16(tS + 16 * w, pk);
+        }
+        l += sum.x + sum.y;
+        tmem_wait_st();
+        tc_fence_before();
+        attn::mbar_arrive(&bar.p_full[sb]);
+      }
+      if (!ok || !wait_all(&bar.o_done[QT == 2 ? q : 0], (tc - 1) & 1)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const bool begun = wk.i0 == 0, ended = wk.i1 == k.nt, whole = begun && ended;
+      const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+      uint16_t* dst = a.out + (trow * a.Hq + head) * D;
+      float* slot = ws.slots + (size_t)(2 * c + (begun ? 1 : 0)) * C::PIECE;
+      if (!whole) {
+        slot[row] = m;
+        slot[C::MR + row] = l;
+        if (begun) slot1 = wk.gi * v.Hkv + wk.h, slot_block = k;
+        else slot0 = ended ? 2 : 1;
+      }
+#pragma unroll 1
+      for (int d = 0; d < D; d += 32) {
+        uint32_t o[32];
+        tmem_ld32(tm + lanes + C::TM_O + q * D + d, o);
+        tmem_wait_ld();
+        float x[32];
+#pragma unroll
+        for (int e = 0; e < 32; e++)
+          x[BITS == 4 ? (e & ~7) + nib_pos(e & 7) : e] = __uint_as_float(o[e]);
+        if (whole) {
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; i++)
+                w[i] = (uint32_t)attn::f_to_dt<BF>(x[e + 2 * i] * inv) |
+                       ((uint32_t)attn::f_to_dt<BF>(x[e + 2 * i + 1] * inv) << 16);
+              *reinterpret_cast<uint4*>(dst + d + e) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(slot + 2 * C::MR + ((size_t)((d + e) / 4) * C::MR + row) * 4) =
+                make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        }
+      }
+      tc_fence_before();
+    }
+    if (tid == 0) ws.meta[c] = make_int4(slot1, slot0 | (slot_block.cols << 8), slot_block.row0, slot_block.col0);
+  } else if (warp < C::kSoftWarps + 8) {
+    // ----------------------------------- dequantize K (4 warps) or V (4 warps)
+    const bool is_v = warp >= C::kSoftWarps + 4;
+    const int w4 = (warp - C::kSoftWarps) & 3, r = w4 * 32 + lane;  // key row of the tile
+    uint8_t* base = sm + (is_v ? C::O_V : C::O_K);
+    uint64_t* full = is_v ? bar.v_full : bar.k_full;
+    uint64_t* empty = is_v ? bar.v_empty : bar.k_empty;
+    constexpr int RW = C::CRB / 16;  // 16-byte words of a code row
+    int tc = 0;
+    bool ok = true;
+    for (; wk.valid() && ok; wk.next(a)) {
+      const Block& k = wk.k;
+      const int32_t* table = v.table + (int64_t)k.b * v.table_stride;
+      const int klo = a.window > 0 ? max(0, k.pmin - a.window + 1) : 0;
+      // the row of tile i: position, and its page (-1: nobody sees the row)
+      auto page_of = [&](int i) -> int {
+        if (i >= wk.i1) return -1;
+        const int j = (tile_of(k, i) << 7) + r;
+        if ((j >> 4) > (k.pmax >> 4)) return -1;
+        return __ldg(table + (j >> v.page_shift));
+      };
+      int page = page_of(wk.i0), page_next = page_of(wk.i0 + 1);
+      for (int i = wk.i0; i < wk.i1; i++, tc++) {
+        const int j = (tile_of(k, i) << 7) + r;
+        const bool wanted = j <= k.pmax && (j >= klo || j < a.sinks);
+        const bool here = (j >> 4) <= (k.pmax >> 4);
+        const bool found = page >= 0 && page < v.num_pages;
+        uint4 raw[RW];
+        uint32_t pr[NG];
+        if (wanted && found) {
+          const uint8_t* src = tile_ptr(v, page, wk.h, (j & v.page_mask) >> 4) + (is_v ? C::HALF : 0);
+          const uint4* cw = reinterpret_cast<const uint4*>(src + (j & 15) * C::CRB);
+#pragma unroll
+          for (int e = 0; e < RW; e++) raw[e] = __ldg(cw + e);
+#pragma unroll
+          for (int e = 0; e < NG; e++)
+            pr[e] = __ldg(reinterpret_cast<const uint32_t*>(src + kTileRows * C::CRB + (j & 15) * C::PRB) + e);
+        } else {
+#pragma unroll
+          for (int e = 0; e < RW; e++) raw[e] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+          for (int e = 0; e < NG; e++) pr[e] = 0u;
+        }
+        const unsigned lost = __ballot_sync(0xffffffffu, here && wanted && !found);
+        page = page_next;
+        page_next = page_of(i + 2);
+        const int buf = KB == 2 ? tc & 1 : 0;
+        if (tc >= KB && !wait_all(&empty[buf], (tc / KB - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        uint8_t* dst = base + buf * C::TILE + (r >> 3) * 1024 + (r & 7) * 128;
+#pragma unroll
+        for (int e = 0; e < D / 8; e++) {
+          const Dequant<BITS, BF> dq(pr[e * 8 / GS]);
+          const uint32_t* words = reinterpret_cast<const uint32_t*>(raw) + e * BITS / 4;
+          *reinterpret_cast<uint4*>(dst + (e >> 3) * C::PANEL + (((e & 7) ^ (r & 7)) << 4)) = dq.eight(words);
+        }
+        if (!is_v && lane == 0) {
+          s_bad[(tc & 3) * 4 + w4] = (uint8_t)(((lost & 0xffffu) ? 1 : 0) | ((lost >> 16) ? 2 : 0));
+          if (lost) raise(v);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        attn::mbar_arrive(&full[buf]);
+      }
+    }
+  } else if (lane == 0) {
+    // ------------------------------------------------------------ MMA issue
+    const uint32_t iqk = idesc_for(BF, 128, C::KT, 0), ipv = idesc_for(BF, 128, D, 1);
+    const uint64_t dq0 = desc_sw128(attn::smem_u32(sm + C::O_Q));
+    const uint64_t dk0 = desc_sw128(attn::smem_u32(sm + C::O_K));
+    const uint64_t dv0 = desc_panels(attn::smem_u32(sm + C::O_V), C::PANEL);
+    int tc = 0;
+    bool ok = true;
+    auto qk = [&](int q, int t) {  // S of row tile q, tile t
+      const int buf = KB == 2 ? t & 1 : 0;
+      const uint32_t dS = tm + (QT == 2 ? q : t & 1) * 128;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ks++) {
+        const uint32_t off = (ks >> 2) * C::PANEL + 32 * (ks & 3);
+        umma_ss(dS, dq0 + ((q * C::TILE + off) >> 4), dk0 + ((buf * C::TILE + off) >> 4), iqk, ks ? 1u : 0u);
+      }
+      umma_commit(&bar.s_full[QT == 2 ? q : t & 1]);
+    };
+    auto pv = [&](int q, int t, bool first) {
+      const int buf = KB == 2 ? t & 1 : 0;
+      const uint32_t tP = tm + (QT == 2 ? q : t & 1) * 128;
+#pragma unroll
+      for (int ks = 0; ks < C::KT / 16; ks++)
+        umma_ts(tm + C::TM_O + q * D, tP + 8 * ks, dv0 + ((buf * C::TILE + 2048 * ks) >> 4), ipv,
+                (first && ks == 0) ? 0u : 1u);
+      umma_commit(&bar.o_done[QT == 2 ? q : 0]);
+    };
+    auto kwait = [&](int t) { return wait(&bar.k_full[KB == 2 ? t & 1 : 0], (KB == 2 ? t >> 1 : t) & 1); };
+    auto vwait = [&](int t) { return wait(&bar.v_full[KB == 2 ? t & 1 : 0], (KB == 2 ? t >> 1 : t) & 1); };
+    for (int u = 0; wk.valid() && ok; wk.next(a), u++) {
+      const int n = wk.i1 - wk.i0;
+      for (int q = 0; q < QT; q++) ok = ok && wait(&bar.q_full[q], u & 1);
+      if (!ok || !kwait(tc)) break;
+      tc_fence_after();
+      for (int q = 0; q < QT; q++) qk(q, tc);
+      umma_commit(&bar.k_empty[KB == 2 ? tc & 1 : 0]);
+      for (int i = 0; i < n && ok; i++, tc++) {
+        const bool more = i + 1 < n;
+        if constexpr (QT == 2) {
+          ok = wait(&bar.p_full[0], tc & 1) && vwait(tc);
+          if (!ok) break;
+          tc_fence_after();
+          pv(0, tc, i == 0);
+          if (more) {
+            if (!(ok = kwait(tc + 1))) break;
+            tc_fence_after();
+            qk(0, tc + 1);
+          }
+          if (!(ok = wait(&bar.p_full[1], tc & 1))) break;
+          tc_fence_after();
+          pv(1, tc, i == 0);
+          umma_commit(&bar.v_empty[KB == 2 ? tc & 1 : 0]);
+          if (more) {
+            qk(1, tc + 1);
+            umma_commit(&bar.k_empty[KB == 2 ? (tc + 1) & 1 : 0]);
+          }
+        } else {
+          if (more) {
+            if (!(ok = kwait(tc + 1))) break;
+            tc_fence_after();
+            qk(0, tc + 1);
+            umma_commit(&bar.k_empty[KB == 2 ? (tc + 1) & 1 : 0]);
+          }
+          ok = wait(&bar.p_full[tc & 1], (tc >> 1) & 1) && vwait(tc);
+          if (!ok) break;
+          tc_fence_after();
+          pv(0, tc, i == 0);
+          umma_commit(&bar.v_empty[KB == 2 ? tc & 1 : 0]);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  // column blocks that see no key: zero rows
+  for (long long gi = c; gi < P.NG; gi += gridDim.x) {
+    if (P.tpre[gi + 1] != P.tpre[gi]) continue;
+    const Block k = get_block<C::MR, 7>(a, P, (int)gi);
+    for (int64_t e = tid; e < (int64_t)v.Hkv * k.cols * (D / 2); e += C::kThreads) {
+      const int d = (int)(e % (D / 2)) * 2, x = (int)(e / (D / 2));
+      store_out<1, BF>(a, k, x / k.cols, x % k.cols, d, 0.0f, 0.0f);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == C::kSoftWarps + 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512));
+  }
+}
+
+// Block (c, y): 32 rows of the unit that begins in CTA c and goes on; its
+// pieces are slot 1 of c and slot 0 of the CTAs after it, in that order.  Warp
+// w takes D / 8 columns.
+template <int BITS, int D, int GS, bool BF>
+__global__ void __launch_bounds__(256) chunk_merge_kernel(const AttnArgs a, const Work ws) {
+  using C = Chunk<BITS, D, GS>;
+  constexpr int NV = D / 32;  // float4s a thread holds
+  __shared__ int s_end;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int c = blockIdx.x, n = gridDim.x, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const int4 where = ws.meta[c];
+  if (where.x < 0) return;
+  if (tid == 0) s_end = n - 1;
+  __syncthreads();
+  for (int i = c + 1 + tid; i < n; i += 256)
+    if ((ws.meta[i].y & 255) == 2) atomicMin(&s_end, i);
+  __syncthreads();
+  const int last = s_end;
+  Block k;
+  k.cols = where.y >> 8;
+  k.row0 = where.z;
+  k.col0 = where.w;
+  const int row = blockIdx.y * 32 + lane;
+  float m = kNeg, l = 0.0f;
+  float4 o[NV];
+#pragma unroll
+  for (int i = 0; i < NV; i++) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int i = c; i <= last; i++) {
+    const float* p = ws.slots + (size_t)(i == c ? 2 * c + 1 : 2 * i) * C::PIECE;
+    const float pm = p[row], pl = p[C::MR + row];
+    float4 z[NV];
+#pragma unroll
+    for (int e = 0; e < NV; e++)
+      z[e] = *reinterpret_cast<const float4*>(p + 2 * C::MR + ((size_t)(w * NV + e) * C::MR + row) * 4);
+    const float mn = fmaxf(m, pm), f = ex2(m - mn), g = ex2(pm - mn);
+    m = mn;
+    l = fmaf(g, pl, l * f);
+#pragma unroll
+    for (int e = 0; e < NV; e++) {
+      o[e].x = fmaf(g, z[e].x, o[e].x * f);
+      o[e].y = fmaf(g, z[e].y, o[e].y * f);
+      o[e].z = fmaf(g, z[e].z, o[e].z * f);
+      o[e].w = fmaf(g, z[e].w, o[e].w * f);
+    }
+  }
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  const int h = where.x % a.v.Hkv;
+#pragma unroll
+  for (int e = 0; e < NV; e++) {
+    const int d = (w * NV + e) * 4;
+    store_out<1, BF>(a, k, h, row, d, o[e].x * inv, o[e].y * inv);
+    store_out<1, BF>(a, k, h, row, d + 2, o[e].z * inv, o[e].w * inv);
+  }
+}
+
+template <int BITS, int D, int GS, bool BF>
+int32_t launch_chunk_one(const AttnArgs& a, const Work& ws, int ctas, int dev, cudaStream_t st) {
+  using C = Chunk<BITS, D, GS>;
+  auto kern = chunk_kernel<BITS, D, GS, BF>;
+  auto merge = chunk_merge_kernel<BITS, D, GS, BF>;
+  int32_t rc = kernel_setup(reinterpret_cast<const void*>(kern), C::kThreads, C::SMEM, dev, nullptr);
+  if (rc) return rc;
+  if ((rc = kernel_carveout(reinterpret_cast<const void*>(merge), dev))) return rc;
+  if (ws.tpre) KVQ_CUDA_TRY(launch_pdl(plan_kernel<C::MR, 7>, dim3(1), dim3(1024), 0, st, a, ws));
+  KVQ_CUDA_TRY(launch_pdl(kern, dim3((unsigned)ctas), dim3(C::kThreads), C::SMEM, st, a, ws));
+  KVQ_CUDA_TRY(launch_pdl(merge, dim3((unsigned)ctas, C::MR / 32), dim3(256), 0, st, a, ws));
+  return KVQ_OK;
+}
+
+// Defined for each (bits, dtype) in its own file.
+template <int BITS, bool BF>
+int32_t launch_chunk(const AttnArgs& a, const Work& ws, int ctas, int dev, cudaStream_t st);
+
+template <int BITS, bool BF>
+int32_t launch_chunk_impl(const AttnArgs& a, const Work& ws, int ctas, int dev, cudaStream_t st) {
+#define KVQ_CHUNK(DD, GG) \
+  if (a.v.D == DD && a.v.gs == GG) return launch_chunk_one<BITS, DD, GG, BF>(a, ws, ctas, dev, st);
+  KVQ_CHUNK(64, 32)
+  KVQ_CHUNK(64, 64)
+  KVQ_CHUNK(128, 32)
+  KVQ_CHUNK(128, 64)
+  KVQ_CHUNK(128, 128)
+  KVQ_CHUNK(256, 32)
+  KVQ_CHUNK(256, 64)
+  KVQ_CHUNK(256, 128)
+#undef KVQ_CHUNK
+  return fail(KVQ_ERR_ARG, "paged: unsupported head_dim / group_size");
+}
+
+}  // namespace paged
+}  // namespace kvq

@@ -1,0 +1,13 @@
+// kvq_paged_chunk_b4.cu — the chunk kernels for 4-bit pages, bf16.
+#include "kvq_paged_chunk.cuh"
+
+namespace kvq {
+namespace paged {
+
+template <>
+int32_t launch_chunk<4, true>(const AttnArgs& a, const Work& ws, int ctas, int dev, cudaStream_t st) {
+  return launch_chunk_impl<4, true>(a, ws, ctas, dev, st);
+}
+
+}  // namespace paged
+}  // namespace kvq

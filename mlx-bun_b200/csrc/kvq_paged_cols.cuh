@@ -94,22 +94,24 @@ __device__ __forceinline__ void checked_rows(const View& v, int b, int& row0, in
   }
 }
 
+// KS: log2 of the keys in a list entry (16 here, 128 in the chunk kernel).
+template <int KS>
 __device__ __forceinline__ void block_keys(Block& k, const AttnArgs& a, int len, int n) {
   k.p0 = len - n;
   k.pmin = k.p0 + k.col0 / a.rep;
   k.pmax = k.p0 + (k.col0 + k.cols - 1) / a.rep;
-  const int hi = len == 0 || k.pmax < 0 ? 0 : (k.pmax >> 4) + 1;
+  const int hi = len == 0 || k.pmax < 0 ? 0 : (k.pmax >> KS) + 1;
   k.nsink = k.lo = 0;
   if (a.window > 0) {
     const int first = max(0, k.pmin - a.window + 1);
-    k.lo = min(first >> 4, hi);
-    k.nsink = (int)(((int64_t)min(a.sinks, first) + 15) >> 4);
+    k.lo = min(first >> KS, hi);
+    k.nsink = (int)(((int64_t)min(a.sinks, first) + (1 << KS) - 1) >> KS);
     if (k.nsink >= k.lo) k.nsink = k.lo = 0;
   }
   k.nt = k.nsink + hi - k.lo;
 }
 
-template <int NC>
+template <int NC, int KS = 4>
 __device__ __forceinline__ Block get_block(const AttnArgs& a, const Plan& P, int gi) {
   Block k;
   int cb;
@@ -131,7 +133,7 @@ __device__ __forceinline__ Block get_block(const AttnArgs& a, const Plan& P, int
   checked_rows(a.v, k.b, k.row0, n, len, false);
   k.col0 = cb * NC;
   k.cols = max(0, min(NC, n * a.rep - k.col0));
-  block_keys(k, a, len, n);
+  block_keys<KS>(k, a, len, n);
   return k;
 }
 
@@ -164,7 +166,7 @@ __device__ __forceinline__ long long block_scan(long long x, long long* tmp, lon
 
 // Fill gpre / tpre (room for B + 1 and max_blocks + 1) and return the number of
 // column blocks.  Blocks beyond max_blocks (overlapping cu_rows) are dropped.
-template <int NC>
+template <int NC, int KS = 4>
 __device__ __forceinline__ int build_plan(const AttnArgs& a, int* gpre, long long* tpre,
                                           int max_blocks, long long* tmp, bool report) {
   const View& v = a.v;
@@ -196,7 +198,7 @@ __device__ __forceinline__ int build_plan(const AttnArgs& a, int* gpre, long lon
   const Plan P{gpre, tpre, NG};
   for (int g0 = 0; g0 < NG; g0 += blockDim.x) {
     const int gi = g0 + threadIdx.x;
-    const int nt = gi < NG ? get_block<NC>(a, P, gi).nt : 0;
+    const int nt = gi < NG ? get_block<NC, KS>(a, P, gi).nt : 0;
     const long long e = base + block_scan(nt, tmp, total);
     if (gi < NG) tpre[gi] = e;
     base += total;
@@ -1056,12 +1058,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32) cols_merge_kernel(const Attn
   store_out<NT, BF>(a, k, h, c0 + 1, d, o.y * i1, o.w * i1);
 }
 
-template <int NC>
+template <int NC, int KS>
 __global__ void __launch_bounds__(1024) plan_kernel(const AttnArgs a, const Work ws) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   __shared__ long long tmp[33];
-  const int NG = build_plan<NC>(a, ws.gpre, ws.tpre, ws.max_blocks, tmp, true);
+  const int NG = build_plan<NC, KS>(a, ws.gpre, ws.tpre, ws.max_blocks, tmp, true);
   if (threadIdx.x == 0) *ws.ng = NG;
 }
 
@@ -1084,7 +1086,7 @@ int32_t launch_cols_one(const AttnArgs& a, const Work& ws, int ctas, int dev, cu
   auto kern = cols_kernel<BITS, D, GS, NT, ST, BF>;
   const int32_t rc = kernel_setup(reinterpret_cast<const void*>(kern), C::W * 32, C::SMEM, dev, nullptr);
   if (rc) return rc;
-  if (ws.tpre) KVQ_CUDA_TRY(launch_pdl(plan_kernel<C::NC>, dim3(1), dim3(1024), 0, st, a, ws));
+  if (ws.tpre) KVQ_CUDA_TRY(launch_pdl(plan_kernel<C::NC, 4>, dim3(1), dim3(1024), 0, st, a, ws));
   KVQ_CUDA_TRY(launch_pdl(kern, dim3((unsigned)ctas), dim3(C::W * 32), C::SMEM, st, a, ws));
   auto merge = cols_merge_kernel<BITS, D, GS, NT, ST, BF>;
   const int32_t rm = kernel_carveout(reinterpret_cast<const void*>(merge), dev);
