@@ -49,7 +49,8 @@ struct Chunk {
   static constexpr int O_TMP = (O_PLAN + (kPlanMax + 1) * 12 + 4 + 15) / 16 * 16;
   static constexpr int O_BAR = O_TMP + 34 * 8;
   static constexpr int O_MISC = O_BAR + 24 * 8;  // TMEM address, bad tiles [4][4]
-  static constexpr int SMEM = O_MISC + 64 + 1024;  // + alignment of the swizzled tiles
+  static constexpr int O_WALK = O_MISC + 64;       // the softmax warps' place in the tile list
+  static constexpr int SMEM = O_WALK + 8 * 128 + 1024;  // + alignment of the swizzled tiles
   static constexpr int kSoftWarps = 4 * QT;
   static constexpr int kThreads = (kSoftWarps + 9) * 32;
   static constexpr int TM_O = 256;              // TMEM columns: S at 0 and 128, O from 256
@@ -167,17 +168,35 @@ struct Dequant {
   }
 };
 
+// UMMA with the descriptors' low words (address, leading offset) in registers;
+// the high word (8-row groups 1024 B apart, 128-byte swizzle) is a constant.
+constexpr uint32_t kDescHi = 64u | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void umma_ss_lo(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n"
+      " mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, {%6, %6, %6, %6}, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kDescHi), "r"(0u));
+}
+__device__ __forceinline__ void umma_ts_lo(uint32_t d, uint32_t a_tmem, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, {%6, %6, %6, %6}, p;\n}\n" ::"r"(d),
+      "r"(a_tmem), "r"(b), "r"(idesc), "r"(acc), "n"(kDescHi), "r"(0u));
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+
 // position of list element i of a 4-bit word's eight values
 __device__ __forceinline__ constexpr int nib_pos(int i) { return (i >> 1) + (i & 1) * 4; }
 
 __device__ __forceinline__ uint32_t idesc_for(bool bf, int M, int N, int b_mn_major) {
   return attn::tc::idesc_f16(M, N, b_mn_major) | (bf ? (1u << 7) | (1u << 10) : 0u);
 }
-// MN-major tile of several 64-element panels, PANEL bytes apart
-__device__ __forceinline__ uint64_t desc_panels(uint32_t saddr, uint32_t panel) {
-  return (attn::tc::desc_sw128(saddr) & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(panel >> 4) << 16);
-}
-
 template <int BITS, int D, int GS, bool BF>
 __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
     chunk_kernel(const AttnArgs a, const Work ws) {
@@ -191,6 +210,8 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
   ChunkBars& bar = *reinterpret_cast<ChunkBars*>(sm + C::O_BAR);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(sm + C::O_MISC);
   volatile uint8_t* s_bad = sm + C::O_MISC + 16;  // [4 tiles in flight][4 warps]
+  // [4]: what the MMA warp is to do with a tile (first / last of a segment)
+  volatile int* s_what = reinterpret_cast<volatile int*>(sm + C::O_MISC + 32);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
@@ -231,8 +252,15 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
   const long long act = max(1ll, min((long long)gridDim.x, RT / 2));
   const long long c = blockIdx.x;
   const long long t0 = c < act ? c * RT / act : RT, t1 = c < act ? (c + 1) * RT / act : RT;
-  Walk<BITS, D, GS> wk;
-  wk.start(a, P, t0, t1);
+  // column blocks that see no key: zero rows
+  for (long long gi = c; gi < P.NG; gi += gridDim.x) {
+    if (P.tpre[gi + 1] != P.tpre[gi]) continue;
+    const Block k = get_block<C::MR, 7>(a, P, (int)gi);
+    for (int64_t e = tid; e < (int64_t)v.Hkv * k.cols * (D / 2); e += C::kThreads) {
+      const int d = (int)(e % (D / 2)) * 2, x = (int)(e / (D / 2));
+      store_out<1, BF>(a, k, x / k.cols, x % k.cols, d, 0.0f, 0.0f);
+    }
+  }
   // Bounded; a role that gives up leaves its loop, and the others' waits run
   // out in turn.  The warp-wide form keeps the warp together.
   auto wait = [&](uint64_t* b, int parity) -> bool {
@@ -243,29 +271,33 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
   auto wait_all = [&](uint64_t* b, int parity) -> bool {
     return __all_sync(0xffffffffu, wait(b, parity));
   };
-  int slot1 = -1, slot0 = 0;  // this CTA's pieces (softmax threads)
-  Block slot_block{};
-
   if (warp < C::kSoftWarps) {
     // ------------------------------------------------ softmax: one row a thread
     const int q = warp >> 2, r = (warp & 3) * 32 + lane;  // row tile, row in it
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const float c2 = fabsf(a.scale) * attn::kLog2e;
+    // in shared memory: the row's registers are P's and S's
+    static_assert(sizeof(Walk<BITS, D, GS>) <= 128, "walk");
+    Walk<BITS, D, GS>& wk = *reinterpret_cast<Walk<BITS, D, GS>*>(sm + C::O_WALK + warp * 128);
+    if (lane == 0) wk.start(a, P, t0, t1);
+    __syncwarp();
+    // this CTA's pieces: nothing yet
+    if (tid == 0) ws.meta[c] = make_int4(-1, 0, 0, 0);
+    const float c2 = fmaxf(fabsf(a.scale) * attn::kLog2e, 1e-30f);  // never 0: -inf stays -inf
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
     int tc = 0;  // tiles so far
     bool ok = true;
-    for (int u = 0; wk.valid() && ok; wk.next(a), u++) {
+    while (wk.valid()) {
       const Block& k = wk.k;
       const int row = q * 128 + r;
-      const bool live = row < k.cols;
-      const int col = k.col0 + (live ? row : 0), tok = col / a.rep;
-      const int64_t trow = k.row0 + tok;
-      const int head = wk.h * a.rep + (col - tok * a.rep);
-      const int p = live ? k.p0 + tok : -1;
+      int p;
       {
-        const uint16_t* src = a.q + trow * a.q_row + (int64_t)head * a.q_head;
+        const bool live = row < k.cols;
+        const int col = k.col0 + (live ? row : 0), tok = col / a.rep;
+        const int head = wk.h * a.rep + (col - tok * a.rep);
+        p = live ? k.p0 + tok : -1;
+        const uint16_t* src = a.q + (int64_t)(k.row0 + tok) * a.q_row + (int64_t)head * a.q_head;
         uint8_t* dst = sm + C::O_Q + q * C::TILE;
-#pragma unroll 4
+#pragma unroll 1
         for (int e = 0; e < D / 8; e++) {
           uint16_t x[8];
           if (ws.vec) {
@@ -291,7 +323,8 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         attn::mbar_arrive(&bar.q_full[q]);
       }
       float m = kNeg, l = 0.0f;
-      for (int i = wk.i0; i < wk.i1; i++, tc++) {
+      const int i1 = wk.i1;
+      for (int i = wk.i0; i < i1; i++, tc++) {
         const int sb = QT == 2 ? q : tc & 1;
         const uint32_t tS = tm + lanes + sb * 128;
         if (!wait_all(&bar.s_full[sb], QT == 2 ? tc & 1 : (tc >> 1) & 1)) {
@@ -397,13 +430,23 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       tc_fence_after();
       const bool begun = wk.i0 == 0, ended = wk.i1 == k.nt, whole = begun && ended;
       const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-      uint16_t* dst = a.out + (trow * a.Hq + head) * D;
+      const bool live = row < k.cols;
+      const int col = k.col0 + (live ? row : 0), tok = col / a.rep;
+      uint16_t* dst = a.out + ((int64_t)(k.row0 + tok) * a.Hq + wk.h * a.rep + (col - tok * a.rep)) * D;
       float* slot = ws.slots + (size_t)(2 * c + (begun ? 1 : 0)) * C::PIECE;
       if (!whole) {
         slot[row] = m;
         slot[C::MR + row] = l;
-        if (begun) slot1 = wk.gi * v.Hkv + wk.h, slot_block = k;
-        else slot0 = ended ? 2 : 1;
+        if (tid == 0) {
+          if (begun) {
+            ws.meta[c].x = wk.gi * v.Hkv + wk.h;
+            ws.meta[c].y |= k.cols << 8;
+            ws.meta[c].z = k.row0;
+            ws.meta[c].w = k.col0;
+          } else {
+            ws.meta[c].y |= ended ? 2 : 1;
+          }
+        }
       }
 #pragma unroll 1
       for (int d = 0; d < D; d += 32) {
@@ -434,8 +477,10 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         }
       }
       tc_fence_before();
+      __syncwarp();
+      if (lane == 0) wk.next(a);
+      __syncwarp();
     }
-    if (tid == 0) ws.meta[c] = make_int4(slot1, slot0 | (slot_block.cols << 8), slot_block.row0, slot_block.col0);
   } else if (warp < C::kSoftWarps + 8) {
     // ----------------------------------- dequantize K (4 warps) or V (4 warps)
     const bool is_v = warp >= C::kSoftWarps + 4;
@@ -444,6 +489,8 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
     uint64_t* full = is_v ? bar.v_full : bar.k_full;
     uint64_t* empty = is_v ? bar.v_empty : bar.k_empty;
     constexpr int RW = C::CRB / 16;  // 16-byte words of a code row
+    Walk<BITS, D, GS> wk;
+    wk.start(a, P, t0, t1);
     int tc = 0;
     bool ok = true;
     for (; wk.valid() && ok; wk.next(a)) {
@@ -497,93 +544,96 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         if (!is_v && lane == 0) {
           s_bad[(tc & 3) * 4 + w4] = (uint8_t)(((lost & 0xffffu) ? 1 : 0) | ((lost >> 16) ? 2 : 0));
           if (lost) raise(v);
+          if (w4 == 0) s_what[tc & 3] = (i == wk.i0 ? 1 : 0) | (i + 1 == wk.i1 ? 2 : 0);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         attn::mbar_arrive(&full[buf]);
       }
     }
-  } else if (lane == 0) {
+  } else {
     // ------------------------------------------------------------ MMA issue
     const uint32_t iqk = idesc_for(BF, 128, C::KT, 0), ipv = idesc_for(BF, 128, D, 1);
-    const uint64_t dq0 = desc_sw128(attn::smem_u32(sm + C::O_Q));
-    const uint64_t dk0 = desc_sw128(attn::smem_u32(sm + C::O_K));
-    const uint64_t dv0 = desc_panels(attn::smem_u32(sm + C::O_V), C::PANEL);
-    int tc = 0;
+    // low descriptor words; V's 64-element panels lie PANEL bytes apart
+    const uint32_t dq0 = (attn::smem_u32(sm + C::O_Q) >> 4) | (1u << 16);
+    const uint32_t dk0 = (attn::smem_u32(sm + C::O_K) >> 4) | (1u << 16);
+    const uint32_t dv0 = (attn::smem_u32(sm + C::O_V) >> 4) | ((uint32_t)(C::PANEL >> 4) << 16);
     bool ok = true;
+    // The whole warp runs this role, so that addresses and descriptors stay in
+    // uniform registers; one elected lane issues.
     auto qk = [&](int q, int t) {  // S of row tile q, tile t
       const int buf = KB == 2 ? t & 1 : 0;
       const uint32_t dS = tm + (QT == 2 ? q : t & 1) * 128;
+      if (!elect_one()) return;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ks++) {
         const uint32_t off = (ks >> 2) * C::PANEL + 32 * (ks & 3);
-        umma_ss(dS, dq0 + ((q * C::TILE + off) >> 4), dk0 + ((buf * C::TILE + off) >> 4), iqk, ks ? 1u : 0u);
+        umma_ss_lo(dS, dq0 + ((q * C::TILE + off) >> 4), dk0 + ((buf * C::TILE + off) >> 4), iqk, ks ? 1u : 0u);
       }
       umma_commit(&bar.s_full[QT == 2 ? q : t & 1]);
     };
     auto pv = [&](int q, int t, bool first) {
       const int buf = KB == 2 ? t & 1 : 0;
       const uint32_t tP = tm + (QT == 2 ? q : t & 1) * 128;
+      if (!elect_one()) return;
 #pragma unroll
       for (int ks = 0; ks < C::KT / 16; ks++)
-        umma_ts(tm + C::TM_O + q * D, tP + 8 * ks, dv0 + ((buf * C::TILE + 2048 * ks) >> 4), ipv,
+        umma_ts_lo(tm + C::TM_O + q * D, tP + 8 * ks, dv0 + ((buf * C::TILE + 2048 * ks) >> 4), ipv,
                 (first && ks == 0) ? 0u : 1u);
       umma_commit(&bar.o_done[QT == 2 ? q : 0]);
     };
-    auto kwait = [&](int t) { return wait(&bar.k_full[KB == 2 ? t & 1 : 0], (KB == 2 ? t >> 1 : t) & 1); };
-    auto vwait = [&](int t) { return wait(&bar.v_full[KB == 2 ? t & 1 : 0], (KB == 2 ? t >> 1 : t) & 1); };
-    for (int u = 0; wk.valid() && ok; wk.next(a), u++) {
-      const int n = wk.i1 - wk.i0;
-      for (int q = 0; q < QT; q++) ok = ok && wait(&bar.q_full[q], u & 1);
-      if (!ok || !kwait(tc)) break;
+    auto commit = [&](uint64_t* b) {
+      if (elect_one()) umma_commit(b);
+    };
+    auto kwait = [&](int t) { return wait_all(&bar.k_full[KB == 2 ? t & 1 : 0], (KB == 2 ? t >> 1 : t) & 1); };
+    auto vwait = [&](int t) { return wait_all(&bar.v_full[KB == 2 ? t & 1 : 0], (KB == 2 ? t >> 1 : t) & 1); };
+    // A tile's products S are issued before the turn of its predecessor's P V
+    // ends; `what` says when that predecessor belongs to another unit.
+    auto start = [&](int t, int u) {  // the first tile of a segment
+      for (int q = 0; q < QT; q++)
+        if (!wait_all(&bar.q_full[q], u & 1)) return false;
       tc_fence_after();
-      for (int q = 0; q < QT; q++) qk(q, tc);
-      umma_commit(&bar.k_empty[KB == 2 ? tc & 1 : 0]);
-      for (int i = 0; i < n && ok; i++, tc++) {
-        const bool more = i + 1 < n;
-        if constexpr (QT == 2) {
-          ok = wait(&bar.p_full[0], tc & 1) && vwait(tc);
-          if (!ok) break;
-          tc_fence_after();
-          pv(0, tc, i == 0);
-          if (more) {
-            if (!(ok = kwait(tc + 1))) break;
-            tc_fence_after();
-            qk(0, tc + 1);
-          }
-          if (!(ok = wait(&bar.p_full[1], tc & 1))) break;
-          tc_fence_after();
-          pv(1, tc, i == 0);
-          umma_commit(&bar.v_empty[KB == 2 ? tc & 1 : 0]);
-          if (more) {
-            qk(1, tc + 1);
-            umma_commit(&bar.k_empty[KB == 2 ? (tc + 1) & 1 : 0]);
-          }
-        } else {
-          if (more) {
-            if (!(ok = kwait(tc + 1))) break;
-            tc_fence_after();
-            qk(0, tc + 1);
-            umma_commit(&bar.k_empty[KB == 2 ? (tc + 1) & 1 : 0]);
-          }
-          ok = wait(&bar.p_full[tc & 1], (tc >> 1) & 1) && vwait(tc);
-          if (!ok) break;
-          tc_fence_after();
-          pv(0, tc, i == 0);
-          umma_commit(&bar.v_empty[KB == 2 ? tc & 1 : 0]);
+      for (int q = 0; q < QT; q++) qk(q, t);
+      commit(&bar.k_empty[KB == 2 ? t & 1 : 0]);
+      return true;
+    };
+    const int total = (int)(t1 - t0);
+    int u = 0;
+    for (int tc = 0; tc < total && ok; tc++) {
+      if (tc == 0 && !(kwait(0) && start(0, 0))) break;
+      const int what = s_what[tc & 3];
+      const bool first = what & 1, more = !(what & 2);
+      if constexpr (QT == 2) {
+        // V and the next K are there early; a row tile's P is what it waits for
+        ok = vwait(tc) && (!more || kwait(tc + 1)) && wait_all(&bar.p_full[0], tc & 1);
+        if (!ok) break;
+        tc_fence_after();
+        pv(0, tc, first);
+        if (more) qk(0, tc + 1);
+        if (!(ok = wait_all(&bar.p_full[1], tc & 1))) break;
+        tc_fence_after();
+        pv(1, tc, first);
+        commit(&bar.v_empty[KB == 2 ? tc & 1 : 0]);
+        if (more) {
+          qk(1, tc + 1);
+          commit(&bar.k_empty[KB == 2 ? (tc + 1) & 1 : 0]);
         }
+      } else {
+        if (more) {
+          if (!(ok = kwait(tc + 1))) break;
+          tc_fence_after();
+          qk(0, tc + 1);
+          commit(&bar.k_empty[KB == 2 ? (tc + 1) & 1 : 0]);
+        }
+        ok = vwait(tc) && wait_all(&bar.p_full[tc & 1], (tc >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        pv(0, tc, first);
+        commit(&bar.v_empty[KB == 2 ? tc & 1 : 0]);
       }
+      if (!more && tc + 1 < total) ok = kwait(tc + 1) && start(tc + 1, ++u);
     }
   }
   __syncwarp();
-  // column blocks that see no key: zero rows
-  for (long long gi = c; gi < P.NG; gi += gridDim.x) {
-    if (P.tpre[gi + 1] != P.tpre[gi]) continue;
-    const Block k = get_block<C::MR, 7>(a, P, (int)gi);
-    for (int64_t e = tid; e < (int64_t)v.Hkv * k.cols * (D / 2); e += C::kThreads) {
-      const int d = (int)(e % (D / 2)) * 2, x = (int)(e / (D / 2));
-      store_out<1, BF>(a, k, x / k.cols, x % k.cols, d, 0.0f, 0.0f);
-    }
-  }
   tc_fence_before();
   __syncthreads();
   if (warp == C::kSoftWarps + 8) {
