@@ -10,10 +10,10 @@
 //   * D 64 / 128: MR 256, two row tiles of 128 (TMEM lanes) in turn: the tensor
 //     core works on one while the softmax warps have the other.
 //   * D 256: MR 128 (its O takes 256 TMEM columns), two S buffers instead.
-// Warps: 4 per row tile for the softmax (a thread owns a row, no shuffles), 4
-// that dequantize K, 4 for V (a thread owns a key row and loads the next
-// tile's codes before it waits for its buffer), 1 that issues the MMAs.
-// All hand-offs are mbarriers with bounded waits.
+// Warps: 8 per row tile for the softmax (two threads share a row, 64 keys each;
+// one exchange of the maximum per tile), 7 that dequantize (a thread owns a key
+// row of K or of V; the 32-row blocks K 0-3, V 0-3 of each tile go round), 1
+// that issues the MMAs.  All hand-offs are mbarriers with bounded waits.
 //
 // Roundings: K, V (as a dense cache of the dtype holds them) and the
 // probabilities go through the tensor core in the dtype; logits, statistics
@@ -49,10 +49,13 @@ struct Chunk {
   static constexpr int O_TMP = (O_PLAN + (kPlanMax + 1) * 12 + 4 + 15) / 16 * 16;
   static constexpr int O_BAR = O_TMP + 34 * 8;
   static constexpr int O_MISC = O_BAR + 24 * 8;  // TMEM address, bad tiles [4][4]
-  static constexpr int O_WALK = O_MISC + 64;       // the softmax warps' place in the tile list
-  static constexpr int SMEM = O_WALK + 8 * 128 + 1024;  // + alignment of the swizzled tiles
-  static constexpr int kSoftWarps = 4 * QT;
-  static constexpr int kThreads = (kSoftWarps + 9) * 32;
+  static constexpr int O_WALK = O_MISC + 64;         // the softmax warps' place in the tile list
+  static constexpr int O_MAX = O_WALK + 16 * 128;    // f32 [2 tiles][QT][2 halves][128]
+  static constexpr int SMEM = O_MAX + 2 * QT * 2 * 128 * 4 + 1024;  // + alignment of the tiles
+  static constexpr int kSoftWarps = 8 * QT;
+  static constexpr int kDequantWarps = 7;
+  static constexpr int kMmaWarp = kSoftWarps + kDequantWarps;
+  static constexpr int kThreads = (kMmaWarp + 1) * 32;  // 24 warps of 80 registers, or 16 of 128
   static constexpr int TM_O = 256;              // TMEM columns: S at 0 and 128, O from 256
   static constexpr int PIECE = MR * (D + 2);    // floats: m [MR], l [MR], O [D / 4][MR][4]
   static_assert(SMEM <= 232448, "shared memory");
@@ -61,6 +64,7 @@ struct Chunk {
 struct ChunkBars {
   uint64_t q_full[2], s_full[2], p_full[2], o_done[2];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t x[2][2];  // the exchange of a row tile's halves, alternating
 };
 
 // The segments (runs of tiles inside one unit) of a CTA, walked by each role.
@@ -191,6 +195,28 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+// Wait of at most 2 s; the hint lets the thread sleep in the hardware meanwhile.
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity) {
+  const uint32_t addr = attn::smem_u32(b);
+  uint64_t t0 = 0;
+  for (long long i = 0; i < attn::kWaitLimit; i++) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity), "r"(100000u)
+        : "memory");
+    if (ok) return true;
+    if ((i & 63) == 0) {
+      const uint64_t now = attn::global_ns();
+      if (i == 0) t0 = now;
+      else if (now - t0 > attn::kWaitNs) return false;
+    }
+  }
+  return false;
+}
+
 // position of list element i of a 4-bit word's eight values
 __device__ __forceinline__ constexpr int nib_pos(int i) { return (i >> 1) + (i & 1) * 4; }
 
@@ -215,18 +241,20 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
-      attn::mbar_init(&bar.q_full[i], 128);
+      attn::mbar_init(&bar.q_full[i], 256);
       attn::mbar_init(&bar.s_full[i], 1);
-      attn::mbar_init(&bar.p_full[i], 128);
+      attn::mbar_init(&bar.p_full[i], 256);
       attn::mbar_init(&bar.o_done[i], 1);
       attn::mbar_init(&bar.k_full[i], 128);
       attn::mbar_init(&bar.k_empty[i], 1);
       attn::mbar_init(&bar.v_full[i], 128);
       attn::mbar_init(&bar.v_empty[i], 1);
+      attn::mbar_init(&bar.x[0][i], 256);
+      attn::mbar_init(&bar.x[1][i], 256);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == C::kSoftWarps + 8) {
+  if (warp == C::kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      attn::smem_u32(s_tmem)),
                  "r"(512)
@@ -262,22 +290,31 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
     }
   }
   // Bounded; a role that gives up leaves its loop, and the others' waits run
-  // out in turn.  The warp-wide form keeps the warp together.
-  auto wait = [&](uint64_t* b, int parity) -> bool {
-    if (attn::mbar_wait(b, (uint32_t)parity)) return true;
+  // out in turn.  All lanes together.
+  auto wait_all = [&](uint64_t* b, int parity) -> bool {
+    if (__all_sync(0xffffffffu, bar_wait(b, (uint32_t)parity))) return true;
     raise(v);
     return false;
   };
-  auto wait_all = [&](uint64_t* b, int parity) -> bool {
-    return __all_sync(0xffffffffu, wait(b, parity));
-  };
   if (warp < C::kSoftWarps) {
-    // ------------------------------------------------ softmax: one row a thread
-    const int q = warp >> 2, r = (warp & 3) * 32 + lane;  // row tile, row in it
+    // ------------------------------------- softmax: half a row (64 keys) a thread
+    const int q = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    // in shared memory: the row's registers are P's and S's
+    // in shared memory, to spare registers
     static_assert(sizeof(Walk<BITS, D, GS>) <= 128, "walk");
     Walk<BITS, D, GS>& wk = *reinterpret_cast<Walk<BITS, D, GS>*>(sm + C::O_WALK + warp * 128);
+    float* s_max = reinterpret_cast<float*>(sm + C::O_MAX) + q * 256 + r;  // [half] 128 apart
+    int xc = 0;  // exchanges so far
+    // the other half's value for this row; false: it did not come
+    auto exchange = [&](float& x) -> bool {
+      float* p = s_max + (xc & 1) * QT * 256;
+      p[half * 128] = x;
+      attn::mbar_arrive(&bar.x[q][xc & 1]);
+      const bool there = wait_all(&bar.x[q][xc & 1], (xc >> 1) & 1);
+      xc++;
+      x = p[(half ^ 1) * 128];
+      return there;
+    };
     if (lane == 0) wk.start(a, P, t0, t1);
     __syncwarp();
     // this CTA's pieces: nothing yet
@@ -297,8 +334,8 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         p = live ? k.p0 + tok : -1;
         const uint16_t* src = a.q + (int64_t)(k.row0 + tok) * a.q_row + (int64_t)head * a.q_head;
         uint8_t* dst = sm + C::O_Q + q * C::TILE;
-#pragma unroll 1
-        for (int e = 0; e < D / 8; e++) {
+#pragma unroll 4
+        for (int e = half * (D / 16); e < (half + 1) * (D / 16); e++) {
           uint16_t x[8];
           if (ws.vec) {
             const uint4 y = *reinterpret_cast<const uint4*>(src + e * 8);
@@ -326,33 +363,34 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       const int i1 = wk.i1;
       for (int i = wk.i0; i < i1; i++, tc++) {
         const int sb = QT == 2 ? q : tc & 1;
-        const uint32_t tS = tm + lanes + sb * 128;
+        const uint32_t tS = tm + lanes + sb * 128 + half * 64;  // its 64 keys' columns
         if (!wait_all(&bar.s_full[sb], QT == 2 ? tc & 1 : (tc >> 1) & 1)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const int kb = tile_of(k, i) << 7;
-        const uint32_t bad4 = *reinterpret_cast<volatile uint32_t*>(const_cast<uint8_t*>(s_bad) + (tc & 3) * 4);
-        const bool full = kb + 127 <= k.pmin && bad4 == 0 &&
-                          (a.window == 0 || kb > k.pmax - a.window || kb + 127 < a.sinks);
-        uint32_t vis[4];
+        const int kb = (tile_of(k, i) << 7) + half * 64;
+        const uint32_t bad2 =
+            *reinterpret_cast<volatile uint16_t*>(const_cast<uint8_t*>(s_bad) + (tc & 3) * 4 + half * 2);
+        const bool full = kb + 63 <= k.pmin && bad2 == 0 &&
+                          (a.window == 0 || kb > k.pmax - a.window || kb + 63 < a.sinks);
+        uint32_t vis[2];
         if (!full) {
-          // bits of the tile's keys that this row sees
+          // bits of the keys that this row sees
 #pragma unroll
-          for (int w = 0; w < 4; w++) {
+          for (int w = 0; w < 2; w++) {
             const int j0 = kb + 32 * w;
             auto upto = [](int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); };
             uint32_t x = upto(p + 1 - j0);
             if (a.window > 0) x &= ~upto(p - a.window + 1 - j0) | upto(a.sinks - j0);
-            const uint32_t b2 = (bad4 >> (8 * w)) & 3u;  // two 16-key tiles without a page
+            const uint32_t b2 = (bad2 >> (8 * w)) & 3u;  // two 16-key tiles without a page
             x &= ~(((b2 & 1u) ? 0x0000ffffu : 0u) | ((b2 & 2u) ? 0xffff0000u : 0u));
             vis[w] = x;
           }
         }
         float mx = kNeg;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < 2; w++) {
           uint32_t s[32];
           tmem_ld32(tS + 32 * w, s);
           tmem_wait_ld();
@@ -366,9 +404,14 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
               if ((vis[w] >> e) & 1u) mx = fmaxf(mx, __uint_as_float(s[e]));
           }
         }
+        float other = mx;
+        if (!exchange(other)) {
+          ok = false;
+          break;
+        }
+        mx = fmaxf(mx, other);
         mx = mx > 0.5f * kNeg ? mx * c2 : kNeg;
-        const bool grow = mx > m + 8.0f;
-        if (__any_sync(0xffffffffu, grow)) {
+        if (__any_sync(0xffffffffu, mx > m + 8.0f)) {  // the same for both halves
           const float mn = fmaxf(m, mx), f = ex2(m - mn);
           m = mn;
           l *= f;
@@ -380,7 +423,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
             }
             tc_fence_after();
 #pragma unroll 1
-            for (int d = 0; d < D; d += 32) {
+            for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 32) {
               uint32_t o[32];
               const uint32_t tO = tm + lanes + C::TM_O + q * D + d;
               tmem_ld32(tO, o);
@@ -395,18 +438,19 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         const float2 cc = make_float2(c2, c2), mm = make_float2(-m, -m);
         float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < 2; w++) {
           uint32_t s[32], pk[16];
           tmem_ld32(tS + 32 * w, s);
           tmem_wait_ld();
+          if (!full) {
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+              if (!((vis[w] >> e) & 1u)) s[e] = 0xff800000u;  // -inf: p is 0
+          }
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), cc, mm);
-            float2 y = make_float2(ex2(x.x), ex2(x.y));
-            if (!full) {
-              if (!((vis[w] >> e) & 1u)) y.x = 0.0f;
-              if (!((vis[w] >> (e + 1)) & 1u)) y.y = 0.0f;
-            }
+            const float2 y = make_float2(ex2(x.x), ex2(x.y));
             sum = __fadd2_rn(sum, y);
             if constexpr (BF) {
               const __nv_bfloat162 t = __floats2bfloat162_rn(y.x, y.y);
@@ -415,7 +459,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
               pk[e / 2] = pack_h2(y.x, y.y);
             }
           }
-          // columns 16 w.. of P lie over columns of S that are read already
+          // over columns of S that this thread has read already
           tmem_st16(tS + 16 * w, pk);
         }
         l += sum.x + sum.y;
@@ -428,6 +472,12 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         break;
       }
       tc_fence_after();
+      float rest = l;
+      if (!exchange(rest)) {
+        ok = false;
+        break;
+      }
+      l += rest;
       const bool begun = wk.i0 == 0, ended = wk.i1 == k.nt, whole = begun && ended;
       const float inv = l != 0.0f ? 1.0f / l : 0.0f;
       const bool live = row < k.cols;
@@ -435,8 +485,10 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       uint16_t* dst = a.out + ((int64_t)(k.row0 + tok) * a.Hq + wk.h * a.rep + (col - tok * a.rep)) * D;
       float* slot = ws.slots + (size_t)(2 * c + (begun ? 1 : 0)) * C::PIECE;
       if (!whole) {
-        slot[row] = m;
-        slot[C::MR + row] = l;
+        if (half == 0) {
+          slot[row] = m;
+          slot[C::MR + row] = l;
+        }
         if (tid == 0) {
           if (begun) {
             ws.meta[c].x = wk.gi * v.Hkv + wk.h;
@@ -449,7 +501,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         }
       }
 #pragma unroll 1
-      for (int d = 0; d < D; d += 32) {
+      for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 32) {
         uint32_t o[32];
         tmem_ld32(tm + lanes + C::TM_O + q * D + d, o);
         tmem_wait_ld();
@@ -481,74 +533,86 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       if (lane == 0) wk.next(a);
       __syncwarp();
     }
-  } else if (warp < C::kSoftWarps + 8) {
-    // ----------------------------------- dequantize K (4 warps) or V (4 warps)
-    const bool is_v = warp >= C::kSoftWarps + 4;
-    const int w4 = (warp - C::kSoftWarps) & 3, r = w4 * 32 + lane;  // key row of the tile
-    uint8_t* base = sm + (is_v ? C::O_V : C::O_K);
-    uint64_t* full = is_v ? bar.v_full : bar.k_full;
-    uint64_t* empty = is_v ? bar.v_empty : bar.k_empty;
+  } else if (warp < C::kMmaWarp) {
+    // ------------------------- dequantize: 32-row blocks K 0-3, V 0-3 of each tile
     constexpr int RW = C::CRB / 16;  // 16-byte words of a code row
     Walk<BITS, D, GS> wk;
     wk.start(a, P, t0, t1);
-    int tc = 0;
-    bool ok = true;
-    for (; wk.valid() && ok; wk.next(a)) {
-      const Block& k = wk.k;
-      const int32_t* table = v.table + (int64_t)k.b * v.table_stride;
-      const int klo = a.window > 0 ? max(0, k.pmin - a.window + 1) : 0;
-      // the row of tile i: position, and its page (-1: nobody sees the row)
-      auto page_of = [&](int i) -> int {
-        if (i >= wk.i1) return -1;
-        const int j = (tile_of(k, i) << 7) + r;
-        if ((j >> 4) > (k.pmax >> 4)) return -1;
-        return __ldg(table + (j >> v.page_shift));
-      };
-      int page = page_of(wk.i0), page_next = page_of(wk.i0 + 1);
-      for (int i = wk.i0; i < wk.i1; i++, tc++) {
-        const int j = (tile_of(k, i) << 7) + r;
-        const bool wanted = j <= k.pmax && (j >= klo || j < a.sinks);
-        const bool here = (j >> 4) <= (k.pmax >> 4);
-        const bool found = page >= 0 && page < v.num_pages;
-        uint4 raw[RW];
-        uint32_t pr[NG];
-        if (wanted && found) {
-          const uint8_t* src = tile_ptr(v, page, wk.h, (j & v.page_mask) >> 4) + (is_v ? C::HALF : 0);
-          const uint4* cw = reinterpret_cast<const uint4*>(src + (j & 15) * C::CRB);
-#pragma unroll
-          for (int e = 0; e < RW; e++) raw[e] = __ldg(cw + e);
-#pragma unroll
-          for (int e = 0; e < NG; e++)
-            pr[e] = __ldg(reinterpret_cast<const uint32_t*>(src + kTileRows * C::CRB + (j & 15) * C::PRB) + e);
-        } else {
-#pragma unroll
-          for (int e = 0; e < RW; e++) raw[e] = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-          for (int e = 0; e < NG; e++) pr[e] = 0u;
-        }
-        const unsigned lost = __ballot_sync(0xffffffffu, here && wanted && !found);
-        page = page_next;
-        page_next = page_of(i + 2);
-        const int buf = KB == 2 ? tc & 1 : 0;
-        if (tc >= KB && !wait_all(&empty[buf], (tc / KB - 1) & 1)) {
-          ok = false;
-          break;
-        }
-        uint8_t* dst = base + buf * C::TILE + (r >> 3) * 1024 + (r & 7) * 128;
-#pragma unroll
-        for (int e = 0; e < D / 8; e++) {
-          const Dequant<BITS, BF> dq(pr[e * 8 / GS]);
-          const uint32_t* words = reinterpret_cast<const uint32_t*>(raw) + e * BITS / 4;
-          *reinterpret_cast<uint4*>(dst + (e >> 3) * C::PANEL + (((e & 7) ^ (r & 7)) << 4)) = dq.eight(words);
-        }
-        if (!is_v && lane == 0) {
-          s_bad[(tc & 3) * 4 + w4] = (uint8_t)(((lost & 0xffffu) ? 1 : 0) | ((lost >> 16) ? 2 : 0));
-          if (lost) raise(v);
-          if (w4 == 0) s_what[tc & 3] = (i == wk.i0 ? 1 : 0) | (i + 1 == wk.i1 ? 2 : 0);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        attn::mbar_arrive(&full[buf]);
+    int first = 0;  // tiles of the CTA before the walk's segment
+    const int total = (int)(t1 - t0);
+    // where block n's row lies: list index of its tile, position, page
+    auto seek = [&](int n) {
+      while ((n >> 3) - first >= wk.i1 - wk.i0) {
+        first += wk.i1 - wk.i0;
+        wk.next(a);
       }
+    };
+    auto key_of = [&](int n) { return (tile_of(wk.k, wk.i0 + (n >> 3) - first) << 7) + (n & 3) * 32 + lane; };
+    auto page_of = [&](int j) -> int {  // -1: nobody sees the row
+      if ((j >> 4) > (wk.k.pmax >> 4)) return -1;
+      return __ldg(v.table + (int64_t)wk.k.b * v.table_stride + (j >> v.page_shift));
+    };
+    int n = warp - C::kSoftWarps, j = 0, page = -1;
+    if (n < 8 * total) {
+      seek(n);
+      j = key_of(n);
+      page = page_of(j);
+    }
+    while (n < 8 * total) {
+      const int tc = n >> 3, quarter = n & 3;
+      const bool is_v = n & 4;
+      const Block& k = wk.k;
+      const int klo = a.window > 0 ? max(0, k.pmin - a.window + 1) : 0;
+      const bool wanted = j <= k.pmax && (j >= klo || j < a.sinks);
+      const bool here = (j >> 4) <= (k.pmax >> 4);
+      const bool found = page >= 0 && page < v.num_pages;
+      const int li = wk.i0 + tc - first;
+      const int what = (li == wk.i0 ? 1 : 0) | (li + 1 == wk.i1 ? 2 : 0);
+      uint4 raw[RW];
+      uint32_t pr[NG];
+      if (wanted && found) {
+        const uint8_t* src = tile_ptr(v, page, wk.h, (j & v.page_mask) >> 4) + (is_v ? C::HALF : 0);
+        const uint4* cw = reinterpret_cast<const uint4*>(src + (j & 15) * C::CRB);
+#pragma unroll
+        for (int e = 0; e < RW; e++) raw[e] = __ldg(cw + e);
+#pragma unroll
+        for (int e = 0; e < NG; e++)
+          pr[e] = __ldg(reinterpret_cast<const uint32_t*>(src + kTileRows * C::CRB + (j & 15) * C::PRB) + e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < RW; e++) raw[e] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int e = 0; e < NG; e++) pr[e] = 0u;
+      }
+      const unsigned lost = __ballot_sync(0xffffffffu, here && wanted && !found);
+      // the next block's page, on its way while this one is converted
+      n += C::kDequantWarps;
+      if (n < 8 * total) {
+        seek(n);
+        j = key_of(n);
+        page = page_of(j);
+      }
+      const int buf = KB == 2 ? tc & 1 : 0;
+      // the buffer's last reader was tile tc - KB.  The barriers go by the parity
+      // of that tile even with one buffer: a warp that had no V block for some
+      // tiles may be two releases behind, which one barrier's parity cannot tell.
+      const int was = tc - KB;
+      if (was >= 0 && !wait_all(is_v ? &bar.v_empty[was & 1] : &bar.k_empty[was & 1], (was >> 1) & 1)) break;
+      const int r = quarter * 32 + lane;
+      uint8_t* dst = sm + (is_v ? C::O_V : C::O_K) + buf * C::TILE + (r >> 3) * 1024 + (r & 7) * 128;
+#pragma unroll
+      for (int e = 0; e < D / 8; e++) {
+        const Dequant<BITS, BF> dq(pr[e * 8 / GS]);
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(raw) + e * BITS / 4;
+        *reinterpret_cast<uint4*>(dst + (e >> 3) * C::PANEL + (((e & 7) ^ (r & 7)) << 4)) = dq.eight(words);
+      }
+      if (!is_v && lane == 0) {
+        s_bad[(tc & 3) * 4 + quarter] = (uint8_t)(((lost & 0xffffu) ? 1 : 0) | ((lost >> 16) ? 2 : 0));
+        if (lost) raise(v);
+        if (quarter == 0) s_what[tc & 3] = what;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      attn::mbar_arrive(is_v ? &bar.v_full[buf] : &bar.k_full[buf]);
     }
   } else {
     // ------------------------------------------------------------ MMA issue
@@ -577,7 +641,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       if (!elect_one()) return;
 #pragma unroll
       for (int ks = 0; ks < C::KT / 16; ks++)
-        umma_ts_lo(tm + C::TM_O + q * D, tP + 8 * ks, dv0 + ((buf * C::TILE + 2048 * ks) >> 4), ipv,
+        umma_ts_lo(tm + C::TM_O + q * D, tP + 8 * (ks & 3) + 64 * (ks >> 2), dv0 + ((buf * C::TILE + 2048 * ks) >> 4), ipv,
                 (first && ks == 0) ? 0u : 1u);
       umma_commit(&bar.o_done[QT == 2 ? q : 0]);
     };
@@ -593,7 +657,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         if (!wait_all(&bar.q_full[q], u & 1)) return false;
       tc_fence_after();
       for (int q = 0; q < QT; q++) qk(q, t);
-      commit(&bar.k_empty[KB == 2 ? t & 1 : 0]);
+      commit(&bar.k_empty[t & 1]);
       return true;
     };
     const int total = (int)(t1 - t0);
@@ -612,23 +676,23 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         if (!(ok = wait_all(&bar.p_full[1], tc & 1))) break;
         tc_fence_after();
         pv(1, tc, first);
-        commit(&bar.v_empty[KB == 2 ? tc & 1 : 0]);
+        commit(&bar.v_empty[tc & 1]);
         if (more) {
           qk(1, tc + 1);
-          commit(&bar.k_empty[KB == 2 ? (tc + 1) & 1 : 0]);
+          commit(&bar.k_empty[(tc + 1) & 1]);
         }
       } else {
         if (more) {
           if (!(ok = kwait(tc + 1))) break;
           tc_fence_after();
           qk(0, tc + 1);
-          commit(&bar.k_empty[KB == 2 ? (tc + 1) & 1 : 0]);
+          commit(&bar.k_empty[(tc + 1) & 1]);
         }
         ok = vwait(tc) && wait_all(&bar.p_full[tc & 1], (tc >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
         pv(0, tc, first);
-        commit(&bar.v_empty[KB == 2 ? tc & 1 : 0]);
+        commit(&bar.v_empty[tc & 1]);
       }
       if (!more && tc + 1 < total) ok = kwait(tc + 1) && start(tc + 1, ++u);
     }
@@ -636,7 +700,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == C::kSoftWarps + 8) {
+  if (warp == C::kMmaWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512));
   }

@@ -247,6 +247,10 @@ PREFILL = [
     (F16, 8, 32, 24, 1, 64, 64, [150], [40], 0, 16, 1),
     (F16, 4, 64, 8, 2, 128, 64, [3000, 2100], [520, 1030], 0, 0, 0),
     (BF16, 8, 128, 2, 2, 128, 32, [1300], [1300], 4, 256, 300),
+    # runs of several tiles in several units per CTA, one and two row tiles
+    (BF16, 8, 64, 16, 8, 256, 32, [2000, 1500], [600, 500], 0, 0, 0),
+    (F16, 4, 64, 16, 8, 256, 16, [1900, 700], [700, 300], 2, 512, 20),
+    (F16, 8, 64, 16, 4, 128, 64, [2100, 1500], [700, 600], 0, 0, 0),
 ]
 
 
