@@ -11,11 +11,11 @@
 //     core works on one while the softmax warps have the other.
 //   * D 256: MR 128 (its O takes 256 TMEM columns), two S buffers instead.
 // Warps: 8 per row tile for the softmax (two threads share a row, 64 keys each;
-// one exchange of the maximum per tile), 7 that load (32-row blocks in turn: a
-// unit's Q, then K 0-3, V 0-3 of each tile, dequantized by the thread that owns
-// the key row), 1 that issues the MMAs.  All hand-offs are mbarriers with
-// bounded waits.  A wait tells two neighbouring phases apart only, so a barrier
-// whose waiter may be two releases behind comes in two, taken alternately.
+// one exchange of the maximum per tile), 7 that dequantize (a thread owns a key
+// row of K or of V; the 32-row blocks K 0-3, V 0-3 of each tile go round), 1
+// that issues the MMAs.  All hand-offs are mbarriers with bounded waits.  A wait
+// tells two neighbouring phases apart only, so a barrier whose waiter may be two
+// releases behind comes in two, taken alternately.
 //
 // Roundings: K, V (as a dense cache of the dtype holds them) and the
 // probabilities go through the tensor core in the dtype; logits, statistics
@@ -50,9 +50,9 @@ struct Chunk {
   static constexpr int O_PLAN = O_V + KB * TILE;
   static constexpr int O_TMP = (O_PLAN + (kPlanMax + 1) * 12 + 4 + 15) / 16 * 16;
   static constexpr int O_BAR = O_TMP + 34 * 8;
-  static constexpr int O_MISC = O_BAR + 24 * 8;  // TMEM address, bad tiles [4][4]
-  static constexpr int O_SEG = O_MISC + 64;          // [4] segments on their way
-  static constexpr int O_MAX = O_SEG + 4 * 64;       // f32 [2 tiles][QT][2 halves][128]
+  static constexpr int O_MISC = O_BAR + 40 * 8;  // TMEM address, bad tiles [4][4]
+  static constexpr int O_WALK = O_MISC + 64;         // the softmax warps' place in the tile list
+  static constexpr int O_MAX = O_WALK + 16 * 128;    // f32 [2 tiles][QT][2 halves][128]
   static constexpr int SMEM = O_MAX + 2 * QT * 2 * 128 * 4 + 1024;  // + alignment of the tiles
   static constexpr int kSoftWarps = 8 * QT;
   static constexpr int kDequantWarps = 7;
@@ -64,9 +64,9 @@ struct Chunk {
 };
 
 struct ChunkBars {
-  uint64_t q_full, q_empty[2], s_full[2], p_full[2], o_done[2];
+  uint64_t q_full[2], s_full[2], p_full[2], o_done[2];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t x[2][2];  // the exchange of a row tile's halves, alternating
+  uint64_t x[2][4][2];  // the exchange of two warps with the same rows, alternating
 };
 
 // The segments (runs of tiles inside one unit) of a CTA, walked by each role.
@@ -110,12 +110,6 @@ struct Walk {
     i0 = 0;
     i1 = (int)min((long long)k.nt, left);
   }
-};
-
-// A segment as the loading warps hand it to the softmax warps.
-struct Segment {
-  Block k;
-  int gi, h, i0, i1;
 };
 
 // 8 codes to 8 dtype values code * s + z, one rounding.  4-bit words give them
@@ -246,13 +240,10 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
   volatile uint8_t* s_bad = sm + C::O_MISC + 16;  // [4 tiles in flight][4 warps]
   // [4]: what the MMA warp is to do with a tile (first / last of a segment)
   volatile int* s_what = reinterpret_cast<volatile int*>(sm + C::O_MISC + 32);
-  static_assert(sizeof(Segment) <= 64, "segment");
-  auto segment = [&](int u) -> Segment& { return *reinterpret_cast<Segment*>(sm + C::O_SEG + (u & 3) * 64); };
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
-    attn::mbar_init(&bar.q_full, C::MR);
     for (int i = 0; i < 2; i++) {
-      attn::mbar_init(&bar.q_empty[i], 1);
+      attn::mbar_init(&bar.q_full[i], 256);
       attn::mbar_init(&bar.s_full[i], 1);
       attn::mbar_init(&bar.p_full[i], 256);
       attn::mbar_init(&bar.o_done[i], 1);
@@ -260,8 +251,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       attn::mbar_init(&bar.k_empty[i], 1);
       attn::mbar_init(&bar.v_full[i], 128);
       attn::mbar_init(&bar.v_empty[i], 1);
-      attn::mbar_init(&bar.x[0][i], 256);
-      attn::mbar_init(&bar.x[1][i], 256);
+      for (int w = 0; w < 8; w++) attn::mbar_init(&bar.x[w >> 2][w & 3][i], 64);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -311,37 +301,69 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
     // ------------------------------------- softmax: half a row (64 keys) a thread
     const int q = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    // in shared memory, to spare registers
+    static_assert(sizeof(Walk<BITS, D, GS>) <= 128, "walk");
+    Walk<BITS, D, GS>& wk = *reinterpret_cast<Walk<BITS, D, GS>*>(sm + C::O_WALK + warp * 128);
     float* s_max = reinterpret_cast<float*>(sm + C::O_MAX) + q * 256 + r;  // [half] 128 apart
     int xc = 0;  // exchanges so far
     // the other half's value for this row; false: it did not come
     auto exchange = [&](float& x) -> bool {
       float* p = s_max + (xc & 1) * QT * 256;
       p[half * 128] = x;
-      attn::mbar_arrive(&bar.x[q][xc & 1]);
-      const bool there = wait_all(&bar.x[q][xc & 1], (xc >> 1) & 1);
+      uint64_t* b = &bar.x[q][warp & 3][xc & 1];
+      attn::mbar_arrive(b);
+      const bool there = wait_all(b, (xc >> 1) & 1);
       xc++;
       x = p[(half ^ 1) * 128];
       return there;
     };
+    if (lane == 0) wk.start(a, P, t0, t1);
+    __syncwarp();
     // this CTA's pieces: nothing yet
     if (tid == 0) ws.meta[c] = make_int4(-1, 0, 0, 0);
     const float c2 = fmaxf(fabsf(a.scale) * attn::kLog2e, 1e-30f);  // never 0: -inf stays -inf
-    const int total = (int)(t1 - t0);
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
     int tc = 0;  // tiles so far
     bool ok = true;
-    for (int u = 0; tc < total && ok; u++) {
-      // the segment is described by the time that its first S is there
-      {
-        const int sb = QT == 2 ? q : tc & 1;
-        if (!wait_all(&bar.s_full[sb], QT == 2 ? tc & 1 : (tc >> 1) & 1)) break;
-      }
-      const Segment& sg = segment(u);
-      const Block& k = sg.k;
+    while (wk.valid()) {
+      const Block& k = wk.k;
       const int row = q * 128 + r;
-      const int p = row < k.cols ? k.p0 + (k.col0 + row) / a.rep : -1;
+      int p;
+      {
+        const bool live = row < k.cols;
+        const int col = k.col0 + (live ? row : 0), tok = col / a.rep;
+        const int head = wk.h * a.rep + (col - tok * a.rep);
+        p = live ? k.p0 + tok : -1;
+        const uint16_t* src = a.q + (int64_t)(k.row0 + tok) * a.q_row + (int64_t)head * a.q_head;
+        uint8_t* dst = sm + C::O_Q + q * C::TILE;
+#pragma unroll 4
+        for (int e = half * (D / 16); e < (half + 1) * (D / 16); e++) {
+          uint16_t x[8];
+          if (ws.vec) {
+            const uint4 y = *reinterpret_cast<const uint4*>(src + e * 8);
+            const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = src[e * 8 + i];
+          }
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t lo = x[BITS == 4 ? nib_pos(2 * i) : 2 * i];
+            const uint32_t hi = x[BITS == 4 ? nib_pos(2 * i + 1) : 2 * i + 1];
+            w[i] = live ? (lo | (hi << 16)) ^ flip : 0u;
+          }
+          *reinterpret_cast<uint4*>(dst + (e >> 3) * C::PANEL + sw128(r, (e & 7) * 8)) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        attn::mbar_arrive(&bar.q_full[q]);
+      }
       float m = kNeg, l = 0.0f;
-      const int i1 = sg.i1;
-      for (int i = sg.i0; i < i1; i++, tc++) {
+      const int i1 = wk.i1;
+      for (int i = wk.i0; i < i1; i++, tc++) {
         const int sb = QT == 2 ? q : tc & 1;
         const uint32_t tS = tm + lanes + sb * 128 + half * 64;  // its 64 keys' columns
         if (!wait_all(&bar.s_full[sb], QT == 2 ? tc & 1 : (tc >> 1) & 1)) {
@@ -395,7 +417,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
           const float mn = fmaxf(m, mx), f = ex2(m - mn);
           m = mn;
           l *= f;
-          if (i > sg.i0) {
+          if (i > wk.i0) {
             // every earlier product of this unit must have landed in O
             if (!wait_all(&bar.o_done[QT == 2 ? q : (tc - 1) & 1], QT == 2 ? (tc - 1) & 1 : ((tc - 1) >> 1) & 1)) {
               ok = false;
@@ -458,11 +480,11 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         break;
       }
       l += rest;
-      const bool begun = sg.i0 == 0, ended = i1 == k.nt, whole = begun && ended;
+      const bool begun = wk.i0 == 0, ended = wk.i1 == k.nt, whole = begun && ended;
       const float inv = l != 0.0f ? 1.0f / l : 0.0f;
       const bool live = row < k.cols;
       const int col = k.col0 + (live ? row : 0), tok = col / a.rep;
-      uint16_t* dst = a.out + ((int64_t)(k.row0 + tok) * a.Hq + sg.h * a.rep + (col - tok * a.rep)) * D;
+      uint16_t* dst = a.out + ((int64_t)(k.row0 + tok) * a.Hq + wk.h * a.rep + (col - tok * a.rep)) * D;
       float* slot = ws.slots + (size_t)(2 * c + (begun ? 1 : 0)) * C::PIECE;
       if (!whole) {
         if (half == 0) {
@@ -471,7 +493,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         }
         if (tid == 0) {
           if (begun) {
-            ws.meta[c].x = sg.gi * v.Hkv + sg.h;
+            ws.meta[c].x = wk.gi * v.Hkv + wk.h;
             ws.meta[c].y |= k.cols << 8;
             ws.meta[c].z = k.row0;
             ws.meta[c].w = k.col0;
@@ -509,83 +531,38 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         }
       }
       tc_fence_before();
+      __syncwarp();
+      if (lane == 0) wk.next(a);
+      __syncwarp();
     }
   } else if (warp < C::kMmaWarp) {
-    // --------------- load: 32-row blocks Q of each segment, K 0-3, V 0-3 of each tile
+    // ------------------------- dequantize: 32-row blocks K 0-3, V 0-3 of each tile
     constexpr int RW = C::CRB / 16;  // 16-byte words of a code row
-    constexpr int NQ = C::MR / 32;
-    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
     Walk<BITS, D, GS> wk;
     wk.start(a, P, t0, t1);
-    int u = 0, first = 0;  // segment, and the CTA's tiles before it
-    int at = warp - C::kSoftWarps;  // block of the segment
-    // go to the block's segment; false: no more
-    auto seek = [&]() -> bool {
-      while (wk.valid() && at >= NQ + 8 * (wk.i1 - wk.i0)) {
-        at -= NQ + 8 * (wk.i1 - wk.i0);
+    int first = 0;  // tiles of the CTA before the walk's segment
+    const int total = (int)(t1 - t0);
+    // where block n's row lies: list index of its tile, position, page
+    auto seek = [&](int n) {
+      while ((n >> 3) - first >= wk.i1 - wk.i0) {
         first += wk.i1 - wk.i0;
-        u++;
         wk.next(a);
       }
-      return wk.valid();
     };
-    auto key_of = [&]() { return (tile_of(wk.k, wk.i0 + ((at - NQ) >> 3)) << 7) + ((at - NQ) & 3) * 32 + lane; };
+    auto key_of = [&](int n) { return (tile_of(wk.k, wk.i0 + (n >> 3) - first) << 7) + (n & 3) * 32 + lane; };
     auto page_of = [&](int j) -> int {  // -1: nobody sees the row
       if ((j >> 4) > (wk.k.pmax >> 4)) return -1;
       return __ldg(v.table + (int64_t)wk.k.b * v.table_stride + (j >> v.page_shift));
     };
-    int j = 0, page = -1;
-    bool more = seek();
-    if (more && at >= NQ) {
-      j = key_of();
+    int n = warp - C::kSoftWarps, j = 0, page = -1;
+    if (n < 8 * total) {
+      seek(n);
+      j = key_of(n);
       page = page_of(j);
     }
-    while (more) {
-      if (at < NQ) {
-        // Q rows; the buffer is free when the segment before has its last S
-        if (u > 0 && !wait_all(&bar.q_empty[(u - 1) & 1], ((u - 1) >> 1) & 1)) break;
-        const Block& k = wk.k;
-        if (at == 0 && lane == 0) segment(u) = Segment{k, wk.gi, wk.h, wk.i0, wk.i1};
-        const int row = at * 32 + lane;
-        const bool live = row < k.cols;
-        const int col = k.col0 + (live ? row : 0), tok = col / a.rep;
-        const uint16_t* src = a.q + (int64_t)(k.row0 + tok) * a.q_row +
-                              (int64_t)(wk.h * a.rep + (col - tok * a.rep)) * a.q_head;
-        uint8_t* dst = sm + C::O_Q + (row >> 7) * C::TILE;
-#pragma unroll 4
-        for (int e = 0; e < D / 8; e++) {
-          uint16_t x[8];
-          if (ws.vec) {
-            const uint4 y = *reinterpret_cast<const uint4*>(src + e * 8);
-            const uint32_t w[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = src[e * 8 + i];
-          }
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const uint32_t lo = x[BITS == 4 ? nib_pos(2 * i) : 2 * i];
-            const uint32_t hi = x[BITS == 4 ? nib_pos(2 * i + 1) : 2 * i + 1];
-            w[i] = live ? (lo | (hi << 16)) ^ flip : 0u;
-          }
-          *reinterpret_cast<uint4*>(dst + (e >> 3) * C::PANEL + sw128(row & 127, (e & 7) * 8)) =
-              make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        attn::mbar_arrive(&bar.q_full);
-        at += C::kDequantWarps;
-        more = seek();
-        if (more && at >= NQ) {
-          j = key_of();
-          page = page_of(j);
-        }
-        continue;
-      }
-      const int block = at - NQ, tc = first + (block >> 3), quarter = block & 3;
-      const bool is_v = block & 4;
+    while (n < 8 * total) {
+      const int tc = n >> 3, quarter = n & 3;
+      const bool is_v = n & 4;
       const Block& k = wk.k;
       const int klo = a.window > 0 ? max(0, k.pmin - a.window + 1) : 0;
       const bool wanted = j <= k.pmax && (j >= klo || j < a.sinks);
@@ -611,16 +588,18 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       }
       const unsigned lost = __ballot_sync(0xffffffffu, here && wanted && !found);
       // the next block's page, on its way while this one is converted
-      at += C::kDequantWarps;
-      more = seek();
-      if (more && at >= NQ) {
-        j = key_of();
+      n += C::kDequantWarps;
+      if (n < 8 * total) {
+        seek(n);
+        j = key_of(n);
         page = page_of(j);
       }
-      // the buffer's last reader was tile tc - KB
+      const int buf = KB == 2 ? tc & 1 : 0;
+      // the buffer's last reader was tile tc - KB.  The barriers go by the parity
+      // of that tile even with one buffer: a warp that had no V block for some
+      // tiles may be two releases behind, which one barrier's parity cannot tell.
       const int was = tc - KB;
       if (was >= 0 && !wait_all(is_v ? &bar.v_empty[was & 1] : &bar.k_empty[was & 1], (was >> 1) & 1)) break;
-      const int buf = KB == 2 ? tc & 1 : 0;
       const int r = quarter * 32 + lane;
       uint8_t* dst = sm + (is_v ? C::O_V : C::O_K) + buf * C::TILE + (r >> 3) * 1024 + (r & 7) * 128;
 #pragma unroll
@@ -673,29 +652,25 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
     };
     auto kwait = [&](int t) { return wait_all(&bar.k_full[KB == 2 ? t & 1 : 0], (KB == 2 ? t >> 1 : t) & 1); };
     auto vwait = [&](int t) { return wait_all(&bar.v_full[KB == 2 ? t & 1 : 0], (KB == 2 ? t >> 1 : t) & 1); };
-    // S of the next tile is issued behind P V of this one, across units too.
-    const int total = (int)(t1 - t0);
-    int u = 0, what = 0, next = 0;
-    auto ready = [&](int t) {  // K of tile t, and Q when a segment begins with it
-      if (!kwait(t)) return false;
-      next = s_what[t & 3];
-      return !(next & 1) || wait_all(&bar.q_full, u & 1);
-    };
-    auto issued = [&](int t) {  // every S of tile t is on its way
-      commit(&bar.k_empty[t & 1]);
-      if (next & 2) commit(&bar.q_empty[u++ & 1]);
-    };
-    if (total > 0 && (ok = ready(0))) {
+    // A tile's products S are issued before the turn of its predecessor's P V
+    // ends; `what` says when that predecessor belongs to another unit.
+    auto start = [&](int t, int u) {  // the first tile of a segment
+      for (int q = 0; q < QT; q++)
+        if (!wait_all(&bar.q_full[q], u & 1)) return false;
       tc_fence_after();
-      for (int q = 0; q < QT; q++) qk(q, 0);
-      issued(0);
-    }
+      for (int q = 0; q < QT; q++) qk(q, t);
+      commit(&bar.k_empty[t & 1]);
+      return true;
+    };
+    const int total = (int)(t1 - t0);
+    int u = 0;
     for (int tc = 0; tc < total && ok; tc++) {
-      what = next;
-      const bool first = what & 1, more = tc + 1 < total;
+      if (tc == 0 && !(kwait(0) && start(0, 0))) break;
+      const int what = s_what[tc & 3];
+      const bool first = what & 1, more = !(what & 2);
       if constexpr (QT == 2) {
         // V and the next K are there early; a row tile's P is what it waits for
-        ok = vwait(tc) && (!more || ready(tc + 1)) && wait_all(&bar.p_full[0], tc & 1);
+        ok = vwait(tc) && (!more || kwait(tc + 1)) && wait_all(&bar.p_full[0], tc & 1);
         if (!ok) break;
         tc_fence_after();
         pv(0, tc, first);
@@ -706,14 +681,14 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         commit(&bar.v_empty[tc & 1]);
         if (more) {
           qk(1, tc + 1);
-          issued(tc + 1);
+          commit(&bar.k_empty[(tc + 1) & 1]);
         }
       } else {
         if (more) {
-          if (!(ok = ready(tc + 1))) break;
+          if (!(ok = kwait(tc + 1))) break;
           tc_fence_after();
           qk(0, tc + 1);
-          issued(tc + 1);
+          commit(&bar.k_empty[(tc + 1) & 1]);
         }
         ok = vwait(tc) && wait_all(&bar.p_full[tc & 1], (tc >> 1) & 1);
         if (!ok) break;
@@ -721,6 +696,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         pv(0, tc, first);
         commit(&bar.v_empty[tc & 1]);
       }
+      if (!more && tc + 1 < total) ok = kwait(tc + 1) && start(tc + 1, ++u);
     }
   }
   __syncwarp();
