@@ -52,7 +52,7 @@ struct Chunk {
   static constexpr int O_BAR = O_TMP + 34 * 8;
   static constexpr int O_MISC = O_BAR + 40 * 8;  // TMEM address, bad tiles [4][4]
   static constexpr int O_WALK = O_MISC + 64;         // the softmax warps' place in the tile list
-  static constexpr int O_MAX = O_WALK + 16 * 128;    // f32 [2 tiles][QT][2 halves][128]
+  static constexpr int O_MAX = O_WALK + 16 * 256;    // f32 [2 tiles][QT][2 halves][128]
   static constexpr int SMEM = O_MAX + 2 * QT * 2 * 128 * 4 + 1024;  // + alignment of the tiles
   static constexpr int kSoftWarps = 8 * QT;
   static constexpr int kDequantWarps = 7;
@@ -303,7 +303,10 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     // in shared memory, to spare registers
     static_assert(sizeof(Walk<BITS, D, GS>) <= 128, "walk");
-    Walk<BITS, D, GS>& wk = *reinterpret_cast<Walk<BITS, D, GS>*>(sm + C::O_WALK + warp * 128);
+    // (two places: the segment at hand and the next one)
+    auto place = [&](int u) -> Walk<BITS, D, GS>& {
+      return *reinterpret_cast<Walk<BITS, D, GS>*>(sm + C::O_WALK + warp * 256 + (u & 1) * 128);
+    };
     float* s_max = reinterpret_cast<float*>(sm + C::O_MAX) + q * 256 + r;  // [half] 128 apart
     int xc = 0;  // exchanges so far
     // the other half's value for this row; false: it did not come
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       x = p[(half ^ 1) * 128];
       return there;
     };
-    if (lane == 0) wk.start(a, P, t0, t1);
+    if (lane == 0) place(0).start(a, P, t0, t1);
     __syncwarp();
     // this CTA's pieces: nothing yet
     if (tid == 0) ws.meta[c] = make_int4(-1, 0, 0, 0);
@@ -325,42 +328,53 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
     int tc = 0;  // tiles so far
     bool ok = true;
-    while (wk.valid()) {
-      const Block& k = wk.k;
-      const int row = q * 128 + r;
-      int p;
-      {
-        const bool live = row < k.cols;
-        const int col = k.col0 + (live ? row : 0), tok = col / a.rep;
-        const int head = wk.h * a.rep + (col - tok * a.rep);
-        p = live ? k.p0 + tok : -1;
-        const uint16_t* src = a.q + (int64_t)(k.row0 + tok) * a.q_row + (int64_t)head * a.q_head;
-        uint8_t* dst = sm + C::O_Q + q * C::TILE;
+    const int row = q * 128 + r;
+    // the thread's half of its Q row; returns the row's position
+    auto load_q = [&](const Walk<BITS, D, GS>& w_) -> int {
+      const Block& k = w_.k;
+      const bool live = row < k.cols;
+      const int col = k.col0 + (live ? row : 0), tok = col / a.rep;
+      const int head = w_.h * a.rep + (col - tok * a.rep);
+      const uint16_t* src = a.q + (int64_t)(k.row0 + tok) * a.q_row + (int64_t)head * a.q_head;
+      uint8_t* dst = sm + C::O_Q + q * C::TILE;
 #pragma unroll 4
-        for (int e = half * (D / 16); e < (half + 1) * (D / 16); e++) {
-          uint16_t x[8];
-          if (ws.vec) {
-            const uint4 y = *reinterpret_cast<const uint4*>(src + e * 8);
-            const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+      for (int e = half * (D / 16); e < (half + 1) * (D / 16); e++) {
+        uint16_t x[8];
+        if (ws.vec) {
+          const uint4 y = *reinterpret_cast<const uint4*>(src + e * 8);
+          const uint32_t w[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-          } else {
+          for (int i = 0; i < 8; i++) x[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+        } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = src[e * 8 + i];
-          }
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const uint32_t lo = x[BITS == 4 ? nib_pos(2 * i) : 2 * i];
-            const uint32_t hi = x[BITS == 4 ? nib_pos(2 * i + 1) : 2 * i + 1];
-            w[i] = live ? (lo | (hi << 16)) ^ flip : 0u;
-          }
-          *reinterpret_cast<uint4*>(dst + (e >> 3) * C::PANEL + sw128(r, (e & 7) * 8)) =
-              make_uint4(w[0], w[1], w[2], w[3]);
+          for (int i = 0; i < 8; i++) x[i] = src[e * 8 + i];
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        attn::mbar_arrive(&bar.q_full[q]);
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const uint32_t lo = x[BITS == 4 ? nib_pos(2 * i) : 2 * i];
+          const uint32_t hi = x[BITS == 4 ? nib_pos(2 * i + 1) : 2 * i + 1];
+          w[i] = live ? (lo | (hi << 16)) ^ flip : 0u;
+        }
+        *reinterpret_cast<uint4*>(dst + (e >> 3) * C::PANEL + sw128(r, (e & 7) * 8)) =
+            make_uint4(w[0], w[1], w[2], w[3]);
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      attn::mbar_arrive(&bar.q_full[q]);
+      return live ? k.p0 + tok : -1;
+    };
+    int p = -1;
+    if (place(0).valid()) p = load_q(place(0));
+    for (int u = 0; place(u).valid(); u++) {
+      const Walk<BITS, D, GS>& wk = place(u);
+      const Block& k = wk.k;
+      // where the CTA goes next, worked out while the first S is on its way
+      __syncwarp();
+      if (lane == 0) {
+        place(u + 1) = wk;
+        place(u + 1).next(a);
+      }
+      __syncwarp();
       float m = kNeg, l = 0.0f;
       const int i1 = wk.i1;
       for (int i = wk.i0; i < i1; i++, tc++) {
@@ -469,6 +483,10 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         tc_fence_before();
         attn::mbar_arrive(&bar.p_full[sb]);
       }
+      // Q is free: this row tile's last S is there.  The next unit's, so that its
+      // first S follows while O is written.
+      int p_next = -1;
+      if (ok && place(u + 1).valid()) p_next = load_q(place(u + 1));
       if (!ok || !wait_all(&bar.o_done[QT == 2 ? q : (tc - 1) & 1], QT == 2 ? (tc - 1) & 1 : ((tc - 1) >> 1) & 1)) {
         ok = false;
         break;
@@ -531,9 +549,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         }
       }
       tc_fence_before();
-      __syncwarp();
-      if (lane == 0) wk.next(a);
-      __syncwarp();
+      p = p_next;
     }
   } else if (warp < C::kMmaWarp) {
     // ------------------------- dequantize: 32-row blocks K 0-3, V 0-3 of each tile
