@@ -45,24 +45,11 @@ __device__ __forceinline__ uint8_t* tile_ptr(const View& v, int page, int h, int
 
 __device__ __forceinline__ void raise(const View& v) { atomicExch(v.status, 1); }
 
-// Rows and first position of sequence b: `n` rows from `row0`, the first of
-// them at position `pos0` (negative when there are more rows than tokens).
+// Rows of sequence b, `n` of them from `row0`, and its length.
 __device__ __forceinline__ void seq_rows(const View& v, int b, int& row0, int& n, int& len) {
   row0 = v.cu ? v.cu[b] : b;
   n = v.cu ? v.cu[b + 1] - row0 : 1;
   len = v.seq_lens[b];
-}
-
-// Sequence of token row t, found by the whole block with one load per 1
-// thread and a counted barrier; v.B when the row is padding.
-__device__ __forceinline__ int block_find_seq(const View& v, int t) {
-  if (!v.cu) return t;
-  int before = 0;
-  for (int b0 = 0; b0 < v.B; b0 += (int)blockDim.x) {
-    const int b = b0 + (int)threadIdx.x;
-    before += __syncthreads_count(b < v.B && v.cu[b + 1] <= t);
-  }
-  return before;
 }
 
 // Host launchers.
