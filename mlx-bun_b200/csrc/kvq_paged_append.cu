@@ -1,12 +1,17 @@
 // kvq_paged_append.cu — RoPE, quantize and write into pages, one launch.
 //
 // Per token row at position p: angle_i = (scale * p) * inv_freq_i and its
-// cosine and sine in 64 bits, (x, y) -> (x cos - y sin, x sin + y cos) in 64
-// bits for K and Q, rounded to 32 bits and then to the dtype; K and V rows
-// then go through the affine group rule of kvq_qrule.cuh into their page.  A
-// 32-bit angle at position 131,072 is off by up to 0.004 rad, more than a
-// bf16 step of the result; and with 64-bit rotation the rounded values, and
-// so the codes, do not depend on the order of operations.
+// cosine and sine in 64 bits, (x, y) -> (x cos - y sin, x sin + y cos) for K and
+// Q to well beyond 32 bits, rounded to 32 bits and then to the dtype; K and V
+// rows then go through the affine group rule of kvq_qrule.cuh into their page.
+// A 32-bit angle at position 131,072 is off by up to 0.004 rad, more than a bf16
+// step of the result; and with products this exact the rounded values, and so
+// the codes, do not depend on how they are computed.
+//
+// The rotation itself is done on pairs of floats (cos = ch + cl, sin = sh + sl,
+// x and y exact): products split by fma, one two-sum, the small terms added at
+// the end, an error of about 2^-46 of the larger product.  64-bit arithmetic
+// would need its conversions, which run at an eighth of the rate.
 //
 // A block takes one to four token rows (their cosines and sines are computed
 // once, in shared memory) and a share of the rows' units; a unit is 8
@@ -34,95 +39,105 @@ __device__ __forceinline__ uint16_t to_bits(float f) {
   if constexpr (BF) return __bfloat16_as_ushort(__float2bfloat16_rn(f));
   else return __half_as_ushort(__float2half_rn(f));
 }
-
-template <bool VEC>
-__device__ __forceinline__ void load8(uint16_t (&x)[8], const uint16_t* p) {
-  if constexpr (VEC) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+template <bool BF>
+__device__ __forceinline__ float2 to_f2(uint32_t w) {
+  if constexpr (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t to_bits2(float2 f) {
+  if constexpr (BF) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
   } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = p[i];
+    const __half2 h = __floats2half2_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
 
-template <bool VEC>
-__device__ __forceinline__ void store8(uint16_t* p, const uint16_t (&x)[8]) {
-  if constexpr (VEC) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) w[i] = (uint32_t)x[2 * i] | ((uint32_t)x[2 * i + 1] << 16);
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) p[i] = x[i];
-  }
-}
-
-// cos / sin of pair i: 8 consecutive pairs are one unit's, so pair i sits at
-// slot (i % 8) * stride + i / 8 and neighbouring lanes read neighbouring slots
+// The angles of one row.  Pairs 2 j and 2 j + 1 share an entry: their cosines'
+// high and low parts in `c`, their sines' in `s` (x, y high; z, w low).  Eight
+// consecutive pairs are one unit's, so entry j sits at slot (j % 4) * stride + j
+// / 4 and neighbouring lanes read neighbouring slots.
+struct Angle2 {
+  float4 c, s;
+};
 struct Table {
-  const double2* cs;
+  const float4 *c, *s;
   int stride;
-  __device__ __forceinline__ double2 at(int i) const { return cs[(i & 7) * stride + (i >> 3)]; }
+  __device__ __forceinline__ Angle2 at2(int j) const {
+    const int k = (j & 3) * stride + (j >> 2);
+    return Angle2{c[k], s[k]};
+  }
 };
 
+// Two pairs at once: x cos + y sin, rounded to 32 bits and then to the dtype
 template <bool BF>
-__device__ __forceinline__ uint16_t round_out(double x) {
-  return to_bits<BF>((float)x);
+__device__ __forceinline__ uint32_t turn2(float2 x, float2 y, const Angle2& a) {
+  const float2 ch = make_float2(a.c.x, a.c.y), cl = make_float2(a.c.z, a.c.w);
+  const float2 sh = make_float2(a.s.x, a.s.y), sl = make_float2(a.s.z, a.s.w);
+  const float2 one = make_float2(-1.0f, -1.0f);
+  const float2 p = __fmul2_rn(x, ch), q = __fmul2_rn(y, sh);
+  const float2 pe = __ffma2_rn(x, ch, make_float2(-p.x, -p.y));
+  const float2 qe = __ffma2_rn(y, sh, make_float2(-q.x, -q.y));
+  const float2 hi = __fadd2_rn(p, q);
+  const float2 b = __ffma2_rn(p, one, hi);    // hi - p
+  const float2 bp = __ffma2_rn(b, one, hi);   // hi - b
+  float2 lo = __fadd2_rn(__ffma2_rn(bp, one, p), __ffma2_rn(b, one, q));
+  lo = __fadd2_rn(lo, __fadd2_rn(pe, qe));
+  lo = __ffma2_rn(x, cl, __ffma2_rn(y, sl, lo));
+  float2 r = __fadd2_rn(hi, lo);
+  // infinite inputs leave no finite remainder
+  if (lo.x != lo.x) r.x = hi.x;
+  if (lo.y != lo.y) r.y = hi.y;
+  return to_bits2<BF>(r);
+}
+// one pair i of the same table
+template <bool BF>
+__device__ __forceinline__ uint16_t turn1(float x, float y, const Table& T, int i) {
+  const Angle2 a = T.at2(i >> 1);
+  return (uint16_t)(turn2<BF>(make_float2(x, x), make_float2(y, y), a) >> (16 * (i & 1)));
 }
 
-// Element e of a row after rotation, x its raw row
-template <bool BF, bool VEC>
-__device__ __forceinline__ void rotate8(uint16_t (&y)[8], const uint16_t* row, int e0,
-                                        const RopeArgs& r, const Table& T) {
-  load8<VEC>(y, row + e0);
-  if (e0 >= r.dims) return;
+// The 8 elements from e0 of a row after rotation; o: their rotation partners
+// (not traditional).  All 8 rotate, in the same half.
+template <bool BF>
+__device__ __forceinline__ void rotate8(uint32_t (&y)[4], const uint32_t (&o)[4], int e0, const RopeArgs& r,
+                                        const Table& T) {
   if (r.traditional) {
+    // words are (x, y) pairs: regroup into two x and two y
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      if (e0 + i < r.dims) {
-        const double2 c = T.at((e0 + i) >> 1);
-        const double a = to_f<BF>(y[i]), b = to_f<BF>(y[i + 1]);
-        y[i] = round_out<BF>(a * c.x - b * c.y);
-        y[i + 1] = round_out<BF>(a * c.y + b * c.x);
-      }
+    for (int i = 0; i < 4; i += 2) {
+      const float2 a = to_f2<BF>(y[i]), b = to_f2<BF>(y[i + 1]);
+      const Angle2 t = T.at2((e0 >> 2) + (i >> 1));
+      const float2 u = make_float2(a.x, b.x), v = make_float2(a.y, b.y);
+      const uint32_t p = turn2<BF>(u, make_float2(-v.x, -v.y), t), q = turn2<BF>(v, u, t);
+      y[i] = __byte_perm(p, q, 0x5410);
+      y[i + 1] = __byte_perm(p, q, 0x7632);
     }
     return;
   }
-  uint16_t z[8];
-  if ((r.half & 7) == 0) {
-    load8<VEC>(z, row + (e0 < r.half ? e0 + r.half : e0 - r.half));
-  } else {
+  const bool lo = e0 < r.half;
+  const int j = (lo ? e0 : e0 - r.half) >> 1;
+  const uint32_t flip = lo ? 0x80008000u : 0u;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int e = e0 + i;
-      z[i] = e < r.dims ? row[e < r.half ? e + r.half : e - r.half] : (uint16_t)0;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const int e = e0 + i;
-    if (e < r.dims) {
-      const bool lo = e < r.half;
-      const double2 c = T.at(lo ? e : e - r.half);
-      const double own = to_f<BF>(y[i]), other = to_f<BF>(z[i]);
-      y[i] = round_out<BF>(lo ? own * c.x - other * c.y : other * c.y + own * c.x);
-    }
-  }
+  for (int i = 0; i < 4; i++)
+    y[i] = turn2<BF>(to_f2<BF>(y[i]), to_f2<BF>(o[i] ^ flip), T.at2(j + i));
 }
 
 // Quantize the 8 elements y of element e0.. of a K or V row; the group's
 // gs / 8 lanes hold its other elements.
 template <bool BF, int BITS>
-__device__ __forceinline__ void quantize8(const uint16_t (&y)[8], int e0, int gs, uint8_t* codes,
+__device__ __forceinline__ void quantize8(const uint32_t (&y)[4], int e0, int gs, uint8_t* codes,
                                           uint8_t* pairs) {
   constexpr float NB = (float)((1 << BITS) - 1);
   float w[8];
 #pragma unroll
-  for (int i = 0; i < 8; i++) w[i] = to_f<BF>(y[i]);
+  for (int i = 0; i < 4; i++) {
+    const float2 f = to_f2<BF>(y[i]);
+    w[2 * i] = f.x;
+    w[2 * i + 1] = f.y;
+  }
   float mn = w[0], mx = w[0];
 #pragma unroll
   for (int i = 1; i < 8; i++) {
@@ -137,10 +152,25 @@ __device__ __forceinline__ void quantize8(const uint16_t (&y)[8], int e0, int gs
   }
   float scale, bias;
   quant_params(mn, mx, NB, scale, bias);
+  // The rule's code is round((w - bias) / scale), half away from zero, of the
+  // IEEE quotient.  With r = 1 / scale the product (w - bias) r is within 2^-22
+  // of the quotient relatively, 6.1e-5 for codes up to 255, so its nearest
+  // integer is the code unless it lies within 1e-4 of a half; only then (ties
+  // of short mantissas, mostly) is the division itself done.  Adding 1.5 2^23
+  // leaves the integer in the low bits of the sum.
+  const float rs = __frcp_rn(scale);
+  constexpr float kMagic = 12582912.0f;
+  constexpr uint32_t kMagicBits = 0x4b400000u;
   uint32_t word[BITS / 4] = {};
+  const bool wide = !(fabsf(scale) < 1e30f);
 #pragma unroll
-  for (int i = 0; i < 8; i++)
-    word[i * BITS / 32] |= quant_code(w[i], scale, bias, NB) << (i * BITS % 32);
+  for (int i = 0; i < 8; i++) {
+    const float q = fminf(fmaxf((w[i] - bias) * rs, 0.0f), NB);
+    const float t = q + kMagic;
+    uint32_t c = __float_as_uint(t) - kMagicBits;
+    if (wide || fabsf(q - (t - kMagic)) > 0.4999f) c = quant_code(w[i], scale, bias, NB);
+    word[i * BITS / 32] |= c << (i * BITS % 32);
+  }
   uint8_t* dst = codes + e0 * BITS / 8;
   if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(dst) = word[0];
   else *reinterpret_cast<uint2*>(dst) = make_uint2(word[0], word[1]);
@@ -149,34 +179,19 @@ __device__ __forceinline__ void quantize8(const uint16_t (&y)[8], int e0, int gs
         (uint32_t)to_bits<BF>(scale) | ((uint32_t)to_bits<BF>(bias) << 16);
 }
 
-// One unit's raw elements: 8 consecutive ones, and 8 rotation partners of them.
-struct Raw {
-  uint4 own, other;
+// What a block knows of its rows: positions, pages, angles.
+struct Shared {
+  float4 c[kMaxRows][kMaxHalf / 2], s[kMaxRows][kMaxHalf / 2];
+  double inv[kMaxHalf];
+  int pos[kMaxRows], page[kMaxRows];  // page: -2 no such row, -1 no page
 };
-__device__ __forceinline__ void unpack(uint16_t (&x)[8], const uint4& u) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 8; i++) x[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-}
 
-// grid (row groups, parts): a block takes R rows from R * blockIdx.x and the
-// units part * kThreads + threadIdx.x, + parts * kThreads, ... of their list.
-// VEC: 16-byte loads, and rotation halves that split into eights; the next
-// unit's loads are then on their way while one is computed.
-template <bool BF, int BITS, bool VEC>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a, const int R) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  __shared__ double2 cs[kMaxRows * kMaxHalf];
-  __shared__ double inv[kMaxHalf];
-  __shared__ int s_pos[kMaxRows], s_page[kMaxRows];  // page: -2 no such row, -1 no page
+// Each row's sequence, position and page by one warp, the frequencies by the
+// others meanwhile; then the angles by all.  Returns the angles' slot stride.
+__device__ __forceinline__ int place_rows(Shared& sh, const AppendArgs& a, int t0, int nr) {
   const View& v = a.v;
   const RopeArgs& r = a.rope;
-  const int t0 = blockIdx.x * R, tid = threadIdx.x, lane = tid & 31;
-  const int nr = min(R, v.rows - t0);
-
-  // Each row's sequence, position and page by one warp, the frequencies by the
-  // others meanwhile.
+  const int tid = threadIdx.x, lane = tid & 31;
   if (tid >> 5 < nr) {
     const int k = tid >> 5, t = t0 + k;
     int b = t;
@@ -201,168 +216,182 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a, co
           }
         }
       }
-      s_pos[k] = pos;
-      s_page[k] = page;
+      sh.pos[k] = pos;
+      sh.page[k] = page;
     }
   }
   for (int i = kThreads - 1 - tid; i < r.half; i += kThreads)
-    inv[i] = r.freqs ? 1.0 / (double)r.freqs[i] : pow(r.base, -2.0 * (double)i / (double)r.dims);
+    sh.inv[i] = r.freqs ? 1.0 / (double)r.freqs[i] : pow(r.base, -2.0 * (double)i / (double)r.dims);
   __syncthreads();
   const int stride = (r.half + 7) >> 3;
   for (int i = tid; i < nr * r.half; i += kThreads) {
-    const int k = i / r.half, e = i - k * r.half;
+    const int k = i / r.half, e = i - k * r.half, j = e >> 1;
     double s, c;
-    sincos((r.scale * (double)s_pos[k]) * inv[e], &s, &c);
-    cs[k * kMaxHalf + (e & 7) * stride + (e >> 3)] = make_double2(c * r.pre, s * r.pre);
+    sincos((r.scale * (double)sh.pos[k]) * sh.inv[e], &s, &c);
+    c *= r.pre;
+    s *= r.pre;
+    const float ch = (float)c, sn = (float)s;
+    const int at = ((j & 3) * stride + (j >> 2)) * 4 + (e & 1);
+    float* pc = reinterpret_cast<float*>(sh.c[k]) + at;
+    float* ps = reinterpret_cast<float*>(sh.s[k]) + at;
+    pc[0] = ch;
+    pc[2] = (float)(c - (double)ch);
+    ps[0] = sn;
+    ps[2] = (float)(s - (double)sn);
   }
   __syncthreads();
+  return stride;
+}
 
+__device__ __forceinline__ void unpack(uint32_t (&x)[4], const uint4& u) {
+  x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+}
+
+// grid (row groups, parts): a block takes R rows from R * blockIdx.x and the
+// units part * kThreads + threadIdx.x, + parts * kThreads, ... of each.  A thread
+// works a unit's place in the row out once, and the next row's loads are on
+// their way while one is computed.  16-byte accesses, rotation halves that split
+// into eights.
+template <bool BF, int BITS, int R>
+__global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ Shared sh;
+  const View& v = a.v;
+  const RopeArgs& r = a.rope;
+  const int t0 = blockIdx.x * R, tid = threadIdx.x, nr = min(R, v.rows - t0);
+  const int stride = place_rows(sh, a, t0, nr);
   const int D = v.D, per_log2 = __ffs(D) - 4;  // units of 8 in a row
   const int kv_units = v.Hkv << per_log2;
   const int crb = code_row_bytes(D, BITS), prb = pair_row_bytes(D, v.gs);
-  // Q units of a head: rotated ones (8 elements and their partners when not
-  // traditional), then the rest of the row, 8 elements each; element by
-  // element when the halves do not split into eights
-  const bool q_vec = VEC || (r.half & 7) == 0;
-  const int q_rot = q_vec ? (r.traditional ? r.dims >> 3 : r.half >> 3) : r.half;
-  const int q_head_units = a.q ? q_rot + (q_vec ? (D - r.dims) >> 3 : D - r.dims) : 0;
+  // Q units of a head: rotated ones, then the rest of the row
+  const int q_rot = r.traditional ? r.dims >> 3 : r.half >> 3;
+  const int q_head_units = a.q ? q_rot + ((D - r.dims) >> 3) : 0;
   const int units = 2 * kv_units + a.Hq * q_head_units;
-  const int padded = (units + 31) & ~31;  // rows start on a warp: groups keep their lanes
-  const int step = gridDim.y * kThreads, end = nr * padded;
-
-  // row k and unit x of list entry u; where its elements lie
-  struct Unit {
-    int k, x, h, e0;
-    bool run;
-    const uint16_t *own, *other;
-  };
-  auto find = [&](int u) {
-    Unit z;
-    z.k = u < end ? u / padded : 0;
-    z.x = u < end ? u - z.k * padded : 0;
-    z.run = u < end && z.x < units && s_page[z.k] != -2;
-    const int64_t t = t0 + z.k;
-    if (z.x < 2 * kv_units || z.x >= units) {
-      const bool is_v = z.x >= kv_units;
-      const int k = z.x >= units ? 0 : (is_v ? z.x - kv_units : z.x);
-      z.h = k >> per_log2;
-      z.e0 = (k - (z.h << per_log2)) << 3;
-      const uint16_t* row = is_v ? a.val + t * a.v_row + z.h * a.v_head : a.k + t * a.k_row + z.h * a.k_head;
-      z.own = row + z.e0;
-      const bool turn = !is_v && !r.traditional && z.e0 < r.dims;
-      z.other = turn ? row + (z.e0 < r.half ? z.e0 + r.half : z.e0 - r.half) : z.own;
+  for (int x = blockIdx.y * kThreads + tid; x < units; x += gridDim.y * kThreads) {
+    const bool is_q = x >= 2 * kv_units, is_v = !is_q && x >= kv_units;
+    int h, e0, other;  // elements from e0, their partners from `other`
+    const uint16_t* src;
+    int64_t row;       // elements between rows
+    bool rot;
+    if (is_q) {
+      const int k = x - 2 * kv_units;
+      h = k / q_head_units;
+      const int j = k - h * q_head_units;
+      rot = j < q_rot;
+      e0 = rot ? j << 3 : r.dims + ((j - q_rot) << 3);
+      other = rot && !r.traditional ? e0 + r.half : e0;
+      src = a.q + h * a.q_head;
+      row = a.q_row;
     } else {
-      const int k = z.x - 2 * kv_units;
-      z.h = k / q_head_units;
-      const int j = k - z.h * q_head_units;
-      const uint16_t* row = a.q + t * a.q_row + z.h * a.q_head;
-      z.e0 = j >= q_rot ? r.dims + ((j - q_rot) << 3) : j << 3;  // (q_vec)
-      z.own = row + z.e0;
-      z.other = j < q_rot && !r.traditional ? z.own + r.half : z.own;
-      if (!q_vec) {
-        z.e0 = j;
-        z.own = z.other = row;
+      const int k = is_v ? x - kv_units : x;
+      h = k >> per_log2;
+      e0 = (k - (h << per_log2)) << 3;
+      rot = !is_v && e0 < r.dims;
+      other = rot && !r.traditional ? (e0 < r.half ? e0 + r.half : e0 - r.half) : e0;
+      src = is_v ? a.val + h * a.v_head : a.k + h * a.k_head;
+      row = is_v ? a.v_row : a.k_row;
+    }
+    src += t0 * row;
+    uint4 own = *reinterpret_cast<const uint4*>(src + e0);
+    uint4 far = *reinterpret_cast<const uint4*>(src + other);
+#pragma unroll 1
+    for (int k = 0; k < nr; k++) {
+      const int page = sh.page[k];
+      const Table T{sh.c[k], sh.s[k], stride};
+      uint32_t y[4], o[4];
+      unpack(y, own);
+      unpack(o, far);
+      if (k + 1 < nr) {
+        src += row;
+        own = *reinterpret_cast<const uint4*>(src + e0);
+        far = *reinterpret_cast<const uint4*>(src + other);
       }
-    }
-    return z;
-  };
-  auto fetch = [&](const Unit& z) {
-    Raw w{};
-    if constexpr (VEC) {
-      w.own = *reinterpret_cast<const uint4*>(z.own);
-      w.other = *reinterpret_cast<const uint4*>(z.other);
-    }
-    return w;
-  };
-  int u = blockIdx.y * kThreads + tid;
-  Unit z = find(u);
-  Raw raw = fetch(z);
-  for (; u < end; u += step) {
-    const Unit cur = z;
-    const Raw w = raw;
-    z = find(u + step);
-    raw = fetch(z);
-    if (!cur.run) continue;
-    const Table T{cs + cur.k * kMaxHalf, stride};
-    const int pos = s_pos[cur.k], page = s_page[cur.k];
-    const int64_t t = t0 + cur.k;
-    uint16_t y[8], o[8];
-    if (cur.x < 2 * kv_units) {
-      const bool is_v = cur.x >= kv_units;
-      if constexpr (VEC) {
-        unpack(y, w.own);
-        if (!is_v && cur.e0 < r.dims) {
-          unpack(o, w.other);
-          if (r.traditional) {
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-              const double2 c = T.at((cur.e0 + i) >> 1);
-              const double p = to_f<BF>(y[i]), q = to_f<BF>(y[i + 1]);
-              y[i] = round_out<BF>(p * c.x - q * c.y);
-              y[i + 1] = round_out<BF>(p * c.y + q * c.x);
-            }
-          } else {
-            const bool lo = cur.e0 < r.half;
-            const int i0 = lo ? cur.e0 : cur.e0 - r.half;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-              const double2 c = T.at(i0 + i);
-              const double own = to_f<BF>(y[i]), other = to_f<BF>(o[i]);
-              y[i] = round_out<BF>(lo ? own * c.x - other * c.y : other * c.y + own * c.x);
-            }
-          }
+      if (page == -2) continue;
+      if (!is_q) {
+        if (rot) rotate8<BF>(y, o, e0, r, T);
+        if (page >= 0) {
+          const int pos = sh.pos[k], pr = pos & (kTileRows - 1);
+          uint8_t* tile = tile_ptr(v, page, h, (pos & v.page_mask) >> 4) + (is_v ? kTileRows * (crb + prb) : 0);
+          quantize8<BF, BITS>(y, e0, v.gs, tile + pr * crb, tile + kTileRows * crb + pr * prb);
         }
-      } else {
-        if (is_v) load8<false>(y, cur.own);
-        else rotate8<BF, false>(y, cur.own - cur.e0, cur.e0, r, T);
+        continue;
+      }
+      uint16_t* dst = a.q_out + ((int64_t)(t0 + k) * a.Hq + h) * D + e0;
+      if (rot && !r.traditional) {
+        uint32_t z[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const Angle2 t = T.at2((e0 >> 1) + i);
+          const float2 p = to_f2<BF>(y[i]), q = to_f2<BF>(o[i]);
+          z[i] = turn2<BF>(q, p, t);
+          y[i] = turn2<BF>(p, make_float2(-q.x, -q.y), t);
+        }
+        *reinterpret_cast<uint4*>(dst + r.half) = make_uint4(z[0], z[1], z[2], z[3]);
+      } else if (rot) {
+        rotate8<BF>(y, y, e0, r, T);
+      }
+      *reinterpret_cast<uint4*>(dst) = make_uint4(y[0], y[1], y[2], y[3]);
+    }
+  }
+}
+
+// Any strides, alignments and rotation sizes: 8 K or V elements, or one Q pair
+// or element, a thread, loaded one by one.  grid (rows, parts).
+template <bool BF, int BITS>
+__global__ void __launch_bounds__(kThreads) append_any_kernel(const AppendArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ Shared sh;
+  const View& v = a.v;
+  const RopeArgs& r = a.rope;
+  const int t = blockIdx.x;
+  const int stride = place_rows(sh, a, t, 1);
+  const int page = sh.page[0], pos = sh.pos[0];
+  if (page == -2) return;
+  const Table T{sh.c[0], sh.s[0], stride};
+  const int D = v.D, per_log2 = __ffs(D) - 4, kv_units = v.Hkv << per_log2;
+  const int crb = code_row_bytes(D, BITS), prb = pair_row_bytes(D, v.gs);
+  const int q_head = a.q ? D - r.half : 0;  // pairs, then the rest of the row
+  const int units = 2 * kv_units + a.Hq * q_head;
+  // element e of a row after rotation
+  auto element = [&](const uint16_t* src, int e) -> uint16_t {
+    if (e >= r.dims) return src[e];
+    const bool first = r.traditional ? !(e & 1) : e < r.half;
+    const int i = r.traditional ? e >> 1 : (first ? e : e - r.half);
+    const float x = to_f<BF>(src[e]), y = to_f<BF>(src[r.traditional ? e ^ 1 : (first ? e + r.half : e - r.half)]);
+    return turn1<BF>(x, first ? -y : y, T, i);
+  };
+  for (int x = blockIdx.y * kThreads + threadIdx.x; x < units; x += gridDim.y * kThreads) {
+    if (x < 2 * kv_units) {
+      const bool is_v = x >= kv_units;
+      const int k = is_v ? x - kv_units : x, h = k >> per_log2, e0 = (k - (h << per_log2)) << 3;
+      const uint16_t* src = is_v ? a.val + t * a.v_row + h * a.v_head : a.k + t * a.k_row + h * a.k_head;
+      uint32_t y[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int e = e0 + 2 * i;
+        y[i] = is_v ? (uint32_t)src[e] | ((uint32_t)src[e + 1] << 16)
+                    : (uint32_t)element(src, e) | ((uint32_t)element(src, e + 1) << 16);
       }
       if (page >= 0) {
-        const int row = pos & (kTileRows - 1);
-        uint8_t* tile = tile_ptr(v, page, cur.h, (pos & v.page_mask) >> 4) + (is_v ? kTileRows * (crb + prb) : 0);
-        quantize8<BF, BITS>(y, cur.e0, v.gs, tile + row * crb, tile + kTileRows * crb + row * prb);
+        const int pr = pos & (kTileRows - 1);
+        uint8_t* tile = tile_ptr(v, page, h, (pos & v.page_mask) >> 4) + (is_v ? kTileRows * (crb + prb) : 0);
+        quantize8<BF, BITS>(y, e0, v.gs, tile + pr * crb, tile + kTileRows * crb + pr * prb);
       }
       continue;
     }
-    uint16_t* dst = a.q_out + (t * a.Hq + cur.h) * D;
-    if (!q_vec) {
-      const int j = cur.e0;
-      const uint16_t* src = cur.own;
-      if (j >= r.half) {
-        dst[r.dims + j - r.half] = src[r.dims + j - r.half];
-      } else {
-        const int i0 = r.traditional ? 2 * j : j, i1 = r.traditional ? 2 * j + 1 : j + r.half;
-        const double2 c = T.at(j);
-        const double x = to_f<BF>(src[i0]), q = to_f<BF>(src[i1]);
-        dst[i0] = round_out<BF>(x * c.x - q * c.y);
-        dst[i1] = round_out<BF>(x * c.y + q * c.x);
-      }
-      continue;
-    }
-    if constexpr (VEC) unpack(y, w.own);
-    else load8<false>(y, cur.own);
-    if (cur.e0 >= r.dims) {
-      store8<VEC>(dst + cur.e0, y);
-    } else if (r.traditional) {
-#pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        const double2 c = T.at((cur.e0 + i) >> 1);
-        const double p = to_f<BF>(y[i]), q = to_f<BF>(y[i + 1]);
-        y[i] = round_out<BF>(p * c.x - q * c.y);
-        y[i + 1] = round_out<BF>(p * c.y + q * c.x);
-      }
-      store8<VEC>(dst + cur.e0, y);
+    const int k = x - 2 * kv_units, h = k / q_head, j = k - h * q_head;
+    const uint16_t* src = a.q + t * a.q_row + h * a.q_head;
+    uint16_t* dst = a.q_out + ((int64_t)t * a.Hq + h) * D;
+    if (j < r.half) {  // both of a pair before either is written: q_out may be q
+      const int i0 = r.traditional ? 2 * j : j, i1 = r.traditional ? 2 * j + 1 : j + r.half;
+      const uint16_t y0 = element(src, i0), y1 = element(src, i1);
+      dst[i0] = y0;
+      dst[i1] = y1;
     } else {
-      if constexpr (VEC) unpack(o, w.other);
-      else load8<false>(o, cur.other);
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const double2 c = T.at(cur.e0 + i);
-        const double x = to_f<BF>(y[i]), q = to_f<BF>(o[i]);
-        y[i] = round_out<BF>(x * c.x - q * c.y);
-        o[i] = round_out<BF>(x * c.y + q * c.x);
-      }
-      store8<VEC>(dst + cur.e0, y);
-      store8<VEC>(dst + cur.e0 + r.half, o);
+      const int e = j - r.half + r.dims;
+      dst[e] = src[e];
     }
   }
 }
@@ -372,28 +401,30 @@ bool vec_ok(const void* p, int64_t row, int64_t head) {
 }
 
 template <bool BF, int BITS>
-int32_t dispatch(bool vec, dim3 grid, cudaStream_t st, const AppendArgs& a, int R) {
-  if (vec) KVQ_CUDA_TRY(launch_pdl(append_kernel<BF, BITS, true>, grid, dim3(kThreads), 0, st, a, R));
-  else KVQ_CUDA_TRY(launch_pdl(append_kernel<BF, BITS, false>, grid, dim3(kThreads), 0, st, a, R));
+int32_t dispatch(bool vec, cudaStream_t st, const AppendArgs& a) {
+  // few rows: one unit per thread, so that a step's latency is one pass; many:
+  // four to a block, whose angles then keep all its threads busy
+  const int units = (2 * a.v.Hkv + (a.q ? a.Hq : 0)) * a.v.D / 8;
+  int parts = 1;
+  while (parts < (units + kThreads - 1) / kThreads && (int64_t)a.v.rows * parts < 296) parts++;
+  const dim3 grid((unsigned)a.v.rows, (unsigned)parts), block(kThreads);
+  if (!vec)
+    KVQ_CUDA_TRY(launch_pdl(append_any_kernel<BF, BITS>, grid, block, 0, st, a));
+  else if (a.v.rows < 148 * 8)
+    KVQ_CUDA_TRY(launch_pdl(append_kernel<BF, BITS, 1>, grid, block, 0, st, a));
+  else
+    KVQ_CUDA_TRY(launch_pdl(append_kernel<BF, BITS, kMaxRows>,
+                            dim3((unsigned)((a.v.rows + kMaxRows - 1) / kMaxRows)), block, 0, st, a));
   return KVQ_OK;
 }
 
 }  // namespace
 
 int32_t launch_paged_append(const AppendArgs& a, cudaStream_t st) {
-  bool vec = vec_ok(a.k, a.k_row, a.k_head) && vec_ok(a.val, a.v_row, a.v_head);
+  bool vec = vec_ok(a.k, a.k_row, a.k_head) && vec_ok(a.val, a.v_row, a.v_head) && a.rope.half % 8 == 0;
   if (a.q) vec = vec && vec_ok(a.q, a.q_row, a.q_head) && vec_ok(a.q_out, 8, 8);
-  vec = vec && a.rope.half % 8 == 0;
-  // few rows: one unit per thread, so that a step's latency is one pass; many:
-  // four to a block, whose angles then keep all its threads busy
-  const int units = (2 * a.v.Hkv + (a.q ? a.Hq : 0)) * a.v.D / 8;
-  const int R = a.v.rows >= 148 * 8 ? kMaxRows : 1;
-  int parts = 1;
-  while (R == 1 && parts < (units + kThreads - 1) / kThreads && (int64_t)a.v.rows * parts < 296) parts++;
-  const dim3 grid((unsigned)((a.v.rows + R - 1) / R), (unsigned)parts);
-  if (a.v.bits == 4)
-    return a.bf16 ? dispatch<true, 4>(vec, grid, st, a, R) : dispatch<false, 4>(vec, grid, st, a, R);
-  return a.bf16 ? dispatch<true, 8>(vec, grid, st, a, R) : dispatch<false, 8>(vec, grid, st, a, R);
+  if (a.v.bits == 4) return a.bf16 ? dispatch<true, 4>(vec, st, a) : dispatch<false, 4>(vec, st, a);
+  return a.bf16 ? dispatch<true, 8>(vec, st, a) : dispatch<false, 8>(vec, st, a);
 }
 
 }  // namespace paged
