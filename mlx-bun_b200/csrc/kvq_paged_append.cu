@@ -127,9 +127,8 @@ __device__ __forceinline__ void rotate8(uint32_t (&y)[4], const uint32_t (&o)[4]
 
 // Quantize the 8 elements y of element e0.. of a K or V row; the group's
 // gs / 8 lanes hold its other elements.
-template <bool BF, int BITS>
-__device__ __forceinline__ void quantize8(const uint32_t (&y)[4], int e0, int gs, uint8_t* codes,
-                                          uint8_t* pairs) {
+template <bool BF, int BITS, int GS>
+__device__ __forceinline__ void quantize8(const uint32_t (&y)[4], int e0, uint8_t* codes, uint8_t* pairs) {
   constexpr float NB = (float)((1 << BITS) - 1);
   float w[8];
 #pragma unroll
@@ -144,8 +143,10 @@ __device__ __forceinline__ void quantize8(const uint32_t (&y)[4], int e0, int gs
     mn = fminf(mn, w[i]);
     mx = fmaxf(mx, w[i]);
   }
-  const int lanes = gs >> 3, lane = threadIdx.x & 31;
+  constexpr int lanes = GS >> 3;
+  const int lane = threadIdx.x & 31;
   const unsigned mask = (0xffffffffu >> (32 - lanes)) << (lane & ~(lanes - 1));
+#pragma unroll
   for (int o = 1; o < lanes; o <<= 1) {
     mn = fminf(mn, __shfl_xor_sync(mask, mn, o));
     mx = fmaxf(mx, __shfl_xor_sync(mask, mx, o));
@@ -162,20 +163,29 @@ __device__ __forceinline__ void quantize8(const uint32_t (&y)[4], int e0, int gs
   constexpr float kMagic = 12582912.0f;
   constexpr uint32_t kMagicBits = 0x4b400000u;
   uint32_t word[BITS / 4] = {};
-  const bool wide = !(fabsf(scale) < 1e30f);
+  unsigned near = fabsf(scale) < 1e30f ? 0u : 0xffu;  // elements to divide
 #pragma unroll
   for (int i = 0; i < 8; i++) {
     const float q = fminf(fmaxf((w[i] - bias) * rs, 0.0f), NB);
     const float t = q + kMagic;
-    uint32_t c = __float_as_uint(t) - kMagicBits;
-    if (wide || fabsf(q - (t - kMagic)) > 0.4999f) c = quant_code(w[i], scale, bias, NB);
-    word[i * BITS / 32] |= c << (i * BITS % 32);
+    if (fabsf(q - (t - kMagic)) > 0.4999f) near |= 1u << i;
+    word[i * BITS / 32] += (__float_as_uint(t) - kMagicBits) << (i * BITS % 32);
+  }
+  while (near) {
+    const int i = __ffs(near) - 1;
+    near &= near - 1;
+    const uint32_t yw = i < 4 ? (i < 2 ? y[0] : y[1]) : (i < 6 ? y[2] : y[3]);
+    const uint32_t c = quant_code(to_f<BF>((uint16_t)(yw >> (16 * (i & 1)))), scale, bias, NB);
+    const int sh = i * BITS % 32;
+#pragma unroll
+    for (int k = 0; k < BITS / 4; k++)
+      if (i * BITS / 32 == k) word[k] = (word[k] & ~(((1u << BITS) - 1u) << sh)) | (c << sh);
   }
   uint8_t* dst = codes + e0 * BITS / 8;
   if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(dst) = word[0];
   else *reinterpret_cast<uint2*>(dst) = make_uint2(word[0], word[1]);
-  if ((e0 & (gs - 1)) == 0)
-    *reinterpret_cast<uint32_t*>(pairs + e0 / gs * 4) =
+  if ((e0 & (GS - 1)) == 0)
+    *reinterpret_cast<uint32_t*>(pairs + e0 / GS * 4) =
         (uint32_t)to_bits<BF>(scale) | ((uint32_t)to_bits<BF>(bias) << 16);
 }
 
@@ -252,7 +262,7 @@ __device__ __forceinline__ void unpack(uint32_t (&x)[4], const uint4& u) {
 // works a unit's place in the row out once, and the next row's loads are on
 // their way while one is computed.  16-byte accesses, rotation halves that split
 // into eights.
-template <bool BF, int BITS, int R>
+template <bool BF, int BITS, int GS, int R>
 __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -313,7 +323,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
         if (page >= 0) {
           const int pos = sh.pos[k], pr = pos & (kTileRows - 1);
           uint8_t* tile = tile_ptr(v, page, h, (pos & v.page_mask) >> 4) + (is_v ? kTileRows * (crb + prb) : 0);
-          quantize8<BF, BITS>(y, e0, v.gs, tile + pr * crb, tile + kTileRows * crb + pr * prb);
+          quantize8<BF, BITS, GS>(y, e0, tile + pr * crb, tile + kTileRows * crb + pr * prb);
         }
         continue;
       }
@@ -338,7 +348,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
 
 // Any strides, alignments and rotation sizes: 8 K or V elements, or one Q pair
 // or element, a thread, loaded one by one.  grid (rows, parts).
-template <bool BF, int BITS>
+template <bool BF, int BITS, int GS>
 __global__ void __launch_bounds__(kThreads) append_any_kernel(const AppendArgs a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -377,7 +387,7 @@ __global__ void __launch_bounds__(kThreads) append_any_kernel(const AppendArgs a
       if (page >= 0) {
         const int pr = pos & (kTileRows - 1);
         uint8_t* tile = tile_ptr(v, page, h, (pos & v.page_mask) >> 4) + (is_v ? kTileRows * (crb + prb) : 0);
-        quantize8<BF, BITS>(y, e0, v.gs, tile + pr * crb, tile + kTileRows * crb + pr * prb);
+        quantize8<BF, BITS, GS>(y, e0, tile + pr * crb, tile + kTileRows * crb + pr * prb);
       }
       continue;
     }
@@ -400,8 +410,8 @@ bool vec_ok(const void* p, int64_t row, int64_t head) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row % 8 == 0 && head % 8 == 0;
 }
 
-template <bool BF, int BITS>
-int32_t dispatch(bool vec, cudaStream_t st, const AppendArgs& a) {
+template <bool BF, int BITS, int GS>
+int32_t launch(bool vec, cudaStream_t st, const AppendArgs& a) {
   // few rows: one unit per thread, so that a step's latency is one pass; many:
   // four to a block, whose angles then keep all its threads busy
   const int units = (2 * a.v.Hkv + (a.q ? a.Hq : 0)) * a.v.D / 8;
@@ -409,13 +419,22 @@ int32_t dispatch(bool vec, cudaStream_t st, const AppendArgs& a) {
   while (parts < (units + kThreads - 1) / kThreads && (int64_t)a.v.rows * parts < 296) parts++;
   const dim3 grid((unsigned)a.v.rows, (unsigned)parts), block(kThreads);
   if (!vec)
-    KVQ_CUDA_TRY(launch_pdl(append_any_kernel<BF, BITS>, grid, block, 0, st, a));
+    KVQ_CUDA_TRY(launch_pdl(append_any_kernel<BF, BITS, GS>, grid, block, 0, st, a));
   else if (a.v.rows < 148 * 8)
-    KVQ_CUDA_TRY(launch_pdl(append_kernel<BF, BITS, 1>, grid, block, 0, st, a));
+    KVQ_CUDA_TRY(launch_pdl(append_kernel<BF, BITS, GS, 1>, grid, block, 0, st, a));
   else
-    KVQ_CUDA_TRY(launch_pdl(append_kernel<BF, BITS, kMaxRows>,
+    KVQ_CUDA_TRY(launch_pdl(append_kernel<BF, BITS, GS, kMaxRows>,
                             dim3((unsigned)((a.v.rows + kMaxRows - 1) / kMaxRows)), block, 0, st, a));
   return KVQ_OK;
+}
+
+template <bool BF, int BITS>
+int32_t dispatch(bool vec, cudaStream_t st, const AppendArgs& a) {
+  switch (a.v.gs) {
+    case 32: return launch<BF, BITS, 32>(vec, st, a);
+    case 64: return launch<BF, BITS, 64>(vec, st, a);
+    default: return launch<BF, BITS, 128>(vec, st, a);
+  }
 }
 
 }  // namespace
