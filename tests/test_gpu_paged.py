@@ -107,6 +107,38 @@ def test_append(case, layout):
     assert torch.equal(q_out.cpu().view(torch.int16), want_q.view(torch.int16))
 
 
+@pytest.mark.parametrize("dt", [F16, BF16], ids=str)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("gs", [32, 64, 128])
+def test_append_quantizes_special_groups(dt, bits, gs):
+    """Constant, tiny, huge and tie-rich groups get the rule's codes, as
+    kvq.quantize gives them and as the oracle does."""
+    gen = torch.Generator().manual_seed(19)
+    d, hkv, page = 128, 2, 16
+    big = 6e4 if dt == F16 else 3e38
+    rows = [torch.zeros(d), torch.full((d,), 0.7), torch.full((d,), -3.0), torch.full((d,), big),
+            torch.arange(d) - 64.0, torch.arange(d) / 16.0, (torch.arange(d) - 40.0) * 0.375,
+            torch.randn(d, generator=gen) * big / 8, torch.randn(d, generator=gen) * 1e-7,
+            torch.randint(-15, 16, (d,), generator=gen) * 0.5, -torch.arange(d).float(),
+            torch.randn(d, generator=gen).clamp(-1, 1)]
+    x = torch.stack(rows).to(dt)[:, None].expand(-1, hkv, -1).contiguous()
+    x[:, 1] = x[:, 1].flip(-1)
+    ref = R.random_pool(gen, 2, page, hkv, d, gs, bits, dt)
+    cache = _cache(ref)
+    table = torch.tensor([[1]], dtype=torch.int32)
+    cache.append(x.cuda(), x.cuda(), table.cuda(), _i32([12]), _i32([0, 12]))
+    ref.put(table[0], torch.arange(12), x, x)
+    # bit for bit, but for the payload of the NaN scales of groups with infinities
+    for got, want in zip(cache.keys + cache.values, (ref.kc, ref.kp, ref.vc, ref.vp)):
+        got = got.cpu()
+        if got.dtype == torch.int32:
+            assert torch.equal(got, want)
+        else:
+            nan = torch.isnan(want)
+            assert torch.equal(torch.isnan(got), nan)
+            assert torch.equal(got.view(torch.int16)[~nan], want.view(torch.int16)[~nan])
+
+
 def test_append_skips_rows_without_a_place():
     """Negative positions, a position past the table and a page outside the
     pool raise the flag and write nothing; the other rows land."""
