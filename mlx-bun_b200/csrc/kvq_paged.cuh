@@ -43,7 +43,10 @@ __device__ __forceinline__ uint8_t* tile_ptr(const View& v, int page, int h, int
   return v.pool + ((((int64_t)page * v.Hkv + h) << v.tiles_shift) + tile) * v.tile_bytes;
 }
 
-__device__ __forceinline__ void raise(const View& v) { atomicExch(v.status, 1); }
+// The pool's error flag: a row, page or length that makes no sense (1), a bounded
+// wait that ran out (2).
+__device__ __forceinline__ void raise(const View& v) { atomicOr(v.status, 1); }
+__device__ __forceinline__ void gave_up(const View& v) { atomicOr(v.status, 2); }
 
 // Rows of sequence b, `n` of them from `row0`, and its length.
 __device__ __forceinline__ void seq_rows(const View& v, int b, int& row0, int& n, int& len) {

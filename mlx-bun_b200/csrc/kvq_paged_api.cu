@@ -1,7 +1,8 @@
 // kvq_paged_api.cu — C entry points of the paged quantized cache: argument
-// checks, workspaces, launches.  Nothing here throws: the arguments are plain
-// values and the only allocation is the stream-ordered workspace.
+// checks, workspaces, launches.
+#include <cmath>
 #include <mutex>
+#include <new>
 #include <string>
 
 #include "kvq_paged.cuh"
@@ -98,6 +99,9 @@ int32_t sdpa(const kvq_paged* c, const kvq_paged_batch* b, bool decode, const vo
   int32_t rc = make_attn(c, b, q_heads, decode, a);
   if (rc) return rc;
   if (window < 0 || sinks < 0) return fail(KVQ_ERR_ARG, "paged: window and sinks must be >= 0");
+  if (!std::isfinite(scale)) return fail(KVQ_ERR_ARG, "paged: scale must be finite");
+  // a window as long as the table holds hides nothing
+  if ((int64_t)window >= ((int64_t)a.v.max_pages << a.v.page_shift)) window = 0;
   if (a.v.rows == 0 || a.v.B == 0) return KVQ_OK;
   if (!q || !q_strides || !out) return fail(KVQ_ERR_ARG, "paged: NULL q / q_strides / out");
   a.q = static_cast<const uint16_t*>(q);
@@ -128,114 +132,141 @@ int32_t sdpa(const kvq_paged* c, const kvq_paged_batch* b, bool decode, const vo
   return rc;
 }
 
+// No exception leaves a C entry (bookkeeping maps and messages allocate).
+template <class F>
+int32_t guarded(F&& f) noexcept {
+  try {
+    return f();
+  } catch (...) {
+    try {
+      return fail(KVQ_ERR_OOM, "out of host memory");
+    } catch (...) {
+      return KVQ_ERR_OOM;
+    }
+  }
+}
+
 }  // namespace
 
 extern "C" {
 
 int32_t kvq_paged_tile_bytes(const kvq_paged* c, size_t* bytes) {
-  if (!bytes) return fail(KVQ_ERR_ARG, "bytes is NULL");
-  static int32_t dummy;
-  if (!c) return fail(KVQ_ERR_ARG, "paged: NULL cache / batch");
-  kvq_paged shape = *c;  // the pool itself need not exist yet
-  shape.pool = reinterpret_cast<void*>(static_cast<uintptr_t>(16));
-  shape.status = &dummy;
-  kvq_paged_batch none{};
-  paged::View v;
-  int32_t rc = make_view(&shape, &none, v);
-  if (rc) return rc;
-  *bytes = (size_t)v.tile_bytes;
-  return KVQ_OK;
+  return guarded([&]() -> int32_t {
+    if (!bytes) return fail(KVQ_ERR_ARG, "bytes is NULL");
+    static int32_t dummy;
+    if (!c) return fail(KVQ_ERR_ARG, "paged: NULL cache / batch");
+    kvq_paged shape = *c;  // the pool itself need not exist yet
+    shape.pool = reinterpret_cast<void*>(static_cast<uintptr_t>(16));
+    shape.status = &dummy;
+    kvq_paged_batch none{};
+    paged::View v;
+    int32_t rc = make_view(&shape, &none, v);
+    if (rc) return rc;
+    *bytes = (size_t)v.tile_bytes;
+    return KVQ_OK;
+  });
 }
 
 int32_t kvq_paged_append(const kvq_paged* c, const kvq_paged_batch* b, const void* k, const void* v,
                          const int64_t* k_strides, const int64_t* v_strides, const kvq_rope* rope,
                          const void* q, int32_t q_heads, const int64_t* q_strides, void* q_out,
                          void* stream) {
-  paged::AppendArgs a{};
-  int32_t rc = make_view(c, b, a.v);
-  if (rc) return rc;
-  if (!a.v.cu && a.v.rows != a.v.B) return fail(KVQ_ERR_ARG, "paged: rows must equal batch without cu_rows");
-  if (q && (q_heads <= 0 || !q_strides || !q_out)) return fail(KVQ_ERR_ARG, "paged: q needs q_heads, q_strides and q_out");
-  if (q && q_out == q &&
-      ((q_heads > 1 && q_strides[1] != a.v.D) || (a.v.rows > 1 && q_strides[0] != (int64_t)q_heads * a.v.D)))
-    return fail(KVQ_ERR_ARG, "paged: q can be rotated in place only when it is contiguous");
-  a.rope.base = 1.0;
-  a.rope.scale = a.rope.pre = 1.0;
-  if (rope) {
-    if (rope->dims < 0 || rope->dims > a.v.D || rope->dims % 2)
-      return fail(KVQ_ERR_ARG, "paged: rope dims must be even and within head_dim");
-    if (rope->dims > 0 && !rope->freqs && !(rope->base > 0.0f))
-      return fail(KVQ_ERR_ARG, "paged: rope base must be positive (or freqs given)");
-    a.rope.dims = rope->dims;
-    a.rope.half = rope->dims / 2;
-    a.rope.traditional = rope->traditional != 0;
-    a.rope.base = rope->base;
-    a.rope.scale = rope->scale != 0.0f ? rope->scale : 1.0f;
-    a.rope.pre = rope->pre_scale != 0.0f ? rope->pre_scale : 1.0f;
-    a.rope.freqs = rope->freqs;
-  }
-  if (a.v.rows == 0 || a.v.B == 0) return KVQ_OK;
-  if (!k || !v || !k_strides || !v_strides) return fail(KVQ_ERR_ARG, "paged: NULL k / v / strides");
-  a.k = static_cast<const uint16_t*>(k);
-  a.val = static_cast<const uint16_t*>(v);
-  a.k_row = k_strides[0];
-  a.k_head = k_strides[1];
-  a.v_row = v_strides[0];
-  a.v_head = v_strides[1];
-  if (q) {
-    a.q = static_cast<const uint16_t*>(q);
-    a.q_row = q_strides[0];
-    a.q_head = q_strides[1];
-    a.q_out = static_cast<uint16_t*>(q_out);
-    a.Hq = q_heads;
-  }
-  a.bf16 = c->dtype == KVQ_DTYPE_BFLOAT16;
-  DeviceGuard guard(c->device);
-  if (!guard.ok) return fail(KVQ_ERR_CUDA, "cannot select the cache's device");
-  return paged::launch_paged_append(a, static_cast<cudaStream_t>(stream));
+  return guarded([&]() -> int32_t {
+    paged::AppendArgs a{};
+    int32_t rc = make_view(c, b, a.v);
+    if (rc) return rc;
+    if (!a.v.cu && a.v.rows != a.v.B) return fail(KVQ_ERR_ARG, "paged: rows must equal batch without cu_rows");
+    if (q && (q_heads <= 0 || !q_strides || !q_out)) return fail(KVQ_ERR_ARG, "paged: q needs q_heads, q_strides and q_out");
+    if (q && q_out == q &&
+        ((q_heads > 1 && q_strides[1] != a.v.D) || (a.v.rows > 1 && q_strides[0] != (int64_t)q_heads * a.v.D)))
+      return fail(KVQ_ERR_ARG, "paged: q can be rotated in place only when it is contiguous");
+    a.rope.base = 1.0;
+    a.rope.scale = a.rope.pre = 1.0;
+    if (rope) {
+      if (rope->dims < 0 || rope->dims > a.v.D || rope->dims % 2)
+        return fail(KVQ_ERR_ARG, "paged: rope dims must be even and within head_dim");
+      if (rope->dims > 0 && !rope->freqs && !(rope->base > 0.0f))
+        return fail(KVQ_ERR_ARG, "paged: rope base must be positive (or freqs given)");
+      a.rope.dims = rope->dims;
+      a.rope.half = rope->dims / 2;
+      a.rope.traditional = rope->traditional != 0;
+      a.rope.base = rope->base;
+      a.rope.scale = rope->scale != 0.0f ? rope->scale : 1.0f;
+      a.rope.pre = rope->pre_scale != 0.0f ? rope->pre_scale : 1.0f;
+      a.rope.freqs = rope->freqs;
+    }
+    if (a.v.rows == 0 || a.v.B == 0) return KVQ_OK;
+    if (!k || !v || !k_strides || !v_strides) return fail(KVQ_ERR_ARG, "paged: NULL k / v / strides");
+    a.k = static_cast<const uint16_t*>(k);
+    a.val = static_cast<const uint16_t*>(v);
+    a.k_row = k_strides[0];
+    a.k_head = k_strides[1];
+    a.v_row = v_strides[0];
+    a.v_head = v_strides[1];
+    if (q) {
+      a.q = static_cast<const uint16_t*>(q);
+      a.q_row = q_strides[0];
+      a.q_head = q_strides[1];
+      a.q_out = static_cast<uint16_t*>(q_out);
+      a.Hq = q_heads;
+    }
+    a.bf16 = c->dtype == KVQ_DTYPE_BFLOAT16;
+    DeviceGuard guard(c->device);
+    if (!guard.ok) return fail(KVQ_ERR_CUDA, "cannot select the cache's device");
+    return paged::launch_paged_append(a, static_cast<cudaStream_t>(stream));
+  });
 }
 
 int32_t kvq_paged_sdpa_workspace(const kvq_paged* c, const kvq_paged_batch* b, int32_t q_heads,
                                  int32_t decode, size_t* bytes) {
-  if (!bytes) return fail(KVQ_ERR_ARG, "bytes is NULL");
-  paged::AttnArgs a;
-  int32_t rc = make_attn(c, b, q_heads, decode != 0, a);
-  if (rc) return rc;
-  DeviceGuard guard(c->device);
-  if (!guard.ok) return fail(KVQ_ERR_CUDA, "cannot select the cache's device");
-  *bytes = paged::paged_attn_workspace(a);
-  return KVQ_OK;
+  return guarded([&]() -> int32_t {
+    if (!bytes) return fail(KVQ_ERR_ARG, "bytes is NULL");
+    paged::AttnArgs a;
+    int32_t rc = make_attn(c, b, q_heads, decode != 0, a);
+    if (rc) return rc;
+    DeviceGuard guard(c->device);
+    if (!guard.ok) return fail(KVQ_ERR_CUDA, "cannot select the cache's device");
+    *bytes = paged::paged_attn_workspace(a);
+    return KVQ_OK;
+  });
 }
 
 int32_t kvq_paged_sdpa_decode(const kvq_paged* c, const kvq_paged_batch* b, const void* q,
                               int32_t q_heads, const int64_t* q_strides, float scale,
                               int32_t window, int32_t sinks, void* out, void* workspace,
                               size_t workspace_bytes, void* stream) {
-  return sdpa(c, b, true, q, q_heads, q_strides, scale, window, sinks, out, workspace,
-              workspace_bytes, stream);
+  return guarded([&]() -> int32_t {
+    return sdpa(c, b, true, q, q_heads, q_strides, scale, window, sinks, out, workspace,
+                workspace_bytes, stream);
+  });
 }
 
 int32_t kvq_paged_sdpa_prefill(const kvq_paged* c, const kvq_paged_batch* b, const void* q,
                                int32_t q_heads, const int64_t* q_strides, float scale,
                                int32_t window, int32_t sinks, void* out, void* workspace,
                                size_t workspace_bytes, void* stream) {
-  return sdpa(c, b, false, q, q_heads, q_strides, scale, window, sinks, out, workspace,
-              workspace_bytes, stream);
+  return guarded([&]() -> int32_t {
+    return sdpa(c, b, false, q, q_heads, q_strides, scale, window, sinks, out, workspace,
+                workspace_bytes, stream);
+  });
 }
 
 int32_t kvq_paged_check(const kvq_paged* c, void* stream) {
-  if (!c || !c->status) return fail(KVQ_ERR_ARG, "paged: NULL cache / status");
-  DeviceGuard guard(c->device);
-  if (!guard.ok) return fail(KVQ_ERR_CUDA, "cannot select the cache's device");
-  KVQ_CUDA_TRY(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)));
-  int flag = 0;
-  KVQ_CUDA_TRY(cudaMemcpy(&flag, c->status, sizeof(int), cudaMemcpyDeviceToHost));
-  if (!flag) return KVQ_OK;
-  const int zero = 0;
-  KVQ_CUDA_TRY(cudaMemcpy(c->status, &zero, sizeof(int), cudaMemcpyHostToDevice));
-  return fail(KVQ_ERR_STATE,
-              "a paged call met a row without a place, a page number outside the pool or a length "
-              "beyond the page table (rows skipped, keys masked)");
+  return guarded([&]() -> int32_t {
+    if (!c || !c->status) return fail(KVQ_ERR_ARG, "paged: NULL cache / status");
+    DeviceGuard guard(c->device);
+    if (!guard.ok) return fail(KVQ_ERR_CUDA, "cannot select the cache's device");
+    KVQ_CUDA_TRY(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)));
+    int flag = 0;
+    KVQ_CUDA_TRY(cudaMemcpy(&flag, c->status, sizeof(int), cudaMemcpyDeviceToHost));
+    if (!flag) return KVQ_OK;
+    const int zero = 0;
+    KVQ_CUDA_TRY(cudaMemcpy(c->status, &zero, sizeof(int), cudaMemcpyHostToDevice));
+    if (flag & 2) return fail(KVQ_ERR_CUDA, "a paged kernel gave up waiting (its results are not valid)");
+    return fail(KVQ_ERR_STATE,
+                "a paged call met a row without a place, a page number outside the pool or a length "
+                "beyond the page table (rows skipped, keys masked)");
+  });
 }
 
 }  // extern "C"

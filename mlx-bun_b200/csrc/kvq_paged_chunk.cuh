@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
   // out in turn.  All lanes together.
   auto wait_all = [&](uint64_t* b, int parity) -> bool {
     if (__all_sync(0xffffffffu, bar_wait(b, (uint32_t)parity))) return true;
-    raise(v);
+    gave_up(v);
     return false;
   };
   if (warp < C::kSoftWarps) {

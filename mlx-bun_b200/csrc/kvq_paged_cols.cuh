@@ -832,7 +832,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, GS, NT, ST>::W * 32, 1)
         __syncwarp();
         if (!attn::mbar_wait(bars + stage, phase)) {
           // give up: wait (bounded) for the copies still in flight, then leave
-          if (lane == 0) raise(v);
+          if (lane == 0) gave_up(v);
           for (int s = 1; s < STAGES; s++) attn::mbar_wait(bars + (stage + s) % STAGES, (stage + s) / STAGES ^ phase);
           left = 0;
           break;

@@ -197,6 +197,61 @@ def test_decode(case):
             assert not got[b].any()
 
 
+@pytest.mark.parametrize("kind", ["decode", "drafts", "chunks"])
+def test_many_sequences(kind):
+    """More sequences and column blocks than a plan in shared memory holds, with
+    empty ones among them, through both attention kernels."""
+    gen = torch.Generator().manual_seed(20)
+    B, page, hq, hkv, d, dt = 600, 16, 8, 2, 64, F16
+    lens = torch.randint(0, 40, (B,), generator=gen).tolist()
+    lens[7] = lens[599] = 0
+    if kind == "decode":
+        rows = [1] * B
+    else:
+        most = 4 if kind == "drafts" else 40
+        rows = [int(torch.randint(0, most + 1, (1,), generator=gen)) for _ in range(B)]
+        if kind == "chunks":  # past 64 rows * heads of a group on average
+            rows = [max(r, 17) for r in rows]
+    pages = _pages(lens, page)
+    ref = R.random_pool(gen, pages, page, hkv, d, 32, 4, dt)
+    table = R.make_table(gen, lens, page, pages)
+    cache = _cache(ref)
+    cu = _cu(rows)
+    q = torch.randn(cu[-1], hq, d, generator=gen).to(dt)
+    if kind == "decode":
+        got = cache.sdpa_decode(q.cuda(), table.cuda(), _i32(lens), 0.2)
+    else:
+        got = cache.sdpa_prefill(q.cuda(), table.cuda(), _i32(lens), _i32(cu), 0.2, 24, 2)
+    cache.check()
+    window = (0, 0) if kind == "decode" else (24, 2)
+    # rows before a sequence's first token see nothing
+    want = [torch.zeros(cu[-1], hq, n, dtype=torch.float64) for n in (d, d, d, 1)]
+    for b, n in enumerate(lens):
+        skip = max(0, rows[b] - n)
+        if rows[b] > skip:
+            r0, r1 = cu[b] + skip, cu[b + 1]
+            for w, x in zip(want, R.attention(ref, q[r0:r1], table[b:b + 1], [n], [0, r1 - r0], 0.2, *window)):
+                w[r0:r1] = x
+    _check(got, *want, dt, dense=kind == "chunks")
+
+
+@pytest.mark.parametrize("window", [64, 65, 2 ** 31 - 1])
+def test_window_as_long_as_the_table(window):
+    gen = torch.Generator().manual_seed(21)
+    ref = R.random_pool(gen, 9, 16, 1, 128, 64, 8, BF16)
+    table = R.make_table(gen, [64, 50], 16, 9, extra=0)
+    cache = _cache(ref)
+    q = torch.randn(90, 2, 128, generator=gen).to(BF16)
+    # 60 rows for 50 tokens: ten of them stand before the first
+    got = cache.sdpa_prefill(q.cuda(), table.cuda(), _i32([64, 50]), _i32([0, 30, 90]), 0.1, window,
+                             2 ** 31 - 1)
+    want = R.attention(ref, q[:30], table[:1], [64], [0, 30], 0.1)
+    _check(got[:30], *want, BF16, dense=True)
+    assert not got[30:40].any()
+    want = R.attention(ref, q[40:], table[1:], [50], [0, 50], 0.1)
+    _check(got[40:], *want, BF16, dense=True)
+
+
 def test_decode_strided_queries_and_table():
     gen = torch.Generator().manual_seed(8)
     lens, page, hq, hkv, d = [70, 35], 16, 8, 2, 128

@@ -31,9 +31,9 @@ def append(p, b, rope=None, q=None, q_heads=0, qs=None, q_out=None, k=4096, v=40
                                        q_out, None)
 
 
-def sdpa(p, b, decode=False, q=4096, q_heads=8, window=0, sinks=0, out=4096):
+def sdpa(p, b, decode=False, q=4096, q_heads=8, window=0, sinks=0, out=4096, scale=1.0):
     fn = _lib.lib().kvq_paged_sdpa_decode if decode else _lib.lib().kvq_paged_sdpa_prefill
-    return fn(ctypes.byref(p), ctypes.byref(b), q, q_heads, S2, 1.0, window, sinks, out, None, 0,
+    return fn(ctypes.byref(p), ctypes.byref(b), q, q_heads, S2, scale, window, sinks, out, None, 0,
               None)
 
 
@@ -103,6 +103,8 @@ def test_bad_attention_arguments():
     assert sdpa(paged(), batch(), window=-1) == _lib.ERR_ARG and "window" in error()
     assert sdpa(paged(), batch(), sinks=-1) == _lib.ERR_ARG
     assert sdpa(paged(), batch(), q=None) == _lib.ERR_ARG
+    assert sdpa(paged(), batch(), scale=float("nan")) == _lib.ERR_ARG and "scale" in error()
+    assert sdpa(paged(), batch(), scale=float("inf")) == _lib.ERR_ARG
     assert sdpa(paged(), batch(), out=None) == _lib.ERR_ARG
     assert sdpa(paged(), batch(), decode=True) == _lib.ERR_ARG  # 5 rows, 2 sequences
     assert "rows must equal batch" in error()
