@@ -239,8 +239,8 @@ struct Cfg {
   static constexpr int O_TMP = (O_PLAN + PLAN_BYTES + 15) / 16 * 16;
   static constexpr int O_BAR = O_TMP + 33 * 8 + 8;
   static constexpr int O_META = O_BAR + W * STAGES * 8;
-  static constexpr int O_INFO = O_META + W * STAGES * TPS * 4;
-  static constexpr int SMEM = O_INFO + W * 2 * 8 + 128;
+  static constexpr int O_INFO = (O_META + W * STAGES * TPS * 4 + 15) / 16 * 16;
+  static constexpr int SMEM = O_INFO + W * 2 * 16 + 128;
   static_assert(PIECE * 4 <= STAGES * STAGE, "a warp's last piece lies in its ring");
   static_assert(SMEM <= 232448, "shared memory");
   static_assert(ST == 1 || (ST == 2 && NT == 1), "two streams share one column tile");
@@ -665,9 +665,10 @@ __device__ __forceinline__ void close(State<BITS, D, GS, NT>& S) {
     }
 }
 
-struct PieceInfo {
-  int unit;   // -1: none
-  int flags;  // 1: begins the unit, 2: ends it
+struct __align__(16) PieceInfo {
+  int unit;        // -1: none
+  int flags;       // 1: begins the unit, 2: ends it; columns << 8
+  int row0, col0;  // of the unit's block
 };
 
 template <int BITS, int D, int GS, int NT, int ST, bool BF>
@@ -688,7 +689,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, GS, NT, ST>::W * 32, 1)
   if (lane == 0)
     for (int s = 0; s < STAGES; s++) attn::mbar_init(bars + s, 1);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  if (lane < 2) info[2 * w + lane] = PieceInfo{-1, 0};
+  if (lane < 2) info[2 * w + lane] = PieceInfo{-1, 0, 0, 0};
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   Plan P;
@@ -892,7 +893,9 @@ __global__ void __launch_bounds__(Cfg<BITS, D, GS, NT, ST>::W * 32, 1)
             *reinterpret_cast<float4*>(dst + 16 * NT + ((k * NT + nn) * 32 + lane) * 4) =
                 make_float4(S.o[k][nn][0], S.o[k][nn][1], S.o[k][nn][2], S.o[k][nn][3]);
         }
-        if (lane == 0) info[2 * w + (begun ? 1 : 0)] = PieceInfo{unit, (begun ? 1 : 0) | (ended ? 2 : 0)};
+        if (lane == 0)
+          info[2 * w + (begun ? 1 : 0)] =
+              PieceInfo{unit, (begun ? 1 : 0) | (ended ? 2 : 0) | (kc.cols << 8), kc.row0, kc.col0};
       }
       if (left > 0) {
         ic = 0;
@@ -912,56 +915,69 @@ __global__ void __launch_bounds__(Cfg<BITS, D, GS, NT, ST>::W * 32, 1)
   __syncthreads();
 
   // combine the CTA's pieces, unit by unit in key order; warp w takes the
-  // fragments w, w + W, ...
-  int slot1 = -1, slot0 = 0;
-  for (int p0 = 0; p0 < 2 * W;) {
-    const PieceInfo first = info[p0];
-    if (first.unit < 0) {
-      p0++;
-      continue;
-    }
-    int p1 = p0 + 1;
-    int flags = first.flags;
-    while (p1 < 2 * W && (info[p1].unit < 0 || info[p1].unit == first.unit)) {
-      if (info[p1].unit >= 0) flags |= info[p1].flags;
-      p1++;
-    }
+  // fragments w, w + W, ..., four pieces' loads at a time
+  static_assert(2 * W <= 32, "a lane per piece");
+  const PieceInfo mine = lane < 2 * W ? info[lane] : PieceInfo{-1, 0, 0, 0};
+  int4 mt = make_int4(-1, 0, 0, 0);  // slot 1's unit, slot 0's state + columns << 8, row, column
+  for (unsigned rest = __ballot_sync(0xffffffffu, mine.unit >= 0); rest;) {
+    const int p0 = __ffs(rest) - 1, unit = __shfl_sync(0xffffffffu, mine.unit, p0);
+    const unsigned chain = __ballot_sync(0xffffffffu, mine.unit == unit);
+    const int flags = __reduce_or_sync(0xffffffffu, mine.unit == unit ? mine.flags & 3 : 0);
+    Block k;
+    k.cols = __shfl_sync(0xffffffffu, mine.flags, p0) >> 8;
+    k.row0 = __shfl_sync(0xffffffffu, mine.row0, p0);
+    k.col0 = __shfl_sync(0xffffffffu, mine.col0, p0);
+    rest &= ~chain;
     auto piece = [&](int p) -> const float* {
       return (p & 1) ? reinterpret_cast<const float*>(smem + (p >> 1) * STAGES * C::STAGE)
                      : reinterpret_cast<const float*>(smem + C::O_PIECE) + (p >> 1) * C::PIECE;
     };
     const bool whole = flags == 3;
-    Block k;
-    if (whole) k = get_block<NC>(a, P, first.unit / v.Hkv);
     float* out_slot = ws.slots + (size_t)(2 * blockIdx.x + ((flags & 1) ? 1 : 0)) * C::PIECE;
     for (int f = w; f < C::FR; f += W) {
       const int nn = f % NT, c0 = nn * 8 + 2 * t;
-      float m0 = kNeg, m1 = kNeg;
-      for (int p = p0; p < p1; p++)
-        if (info[p].unit >= 0) {
-          const float2 x = *reinterpret_cast<const float2*>(piece(p) + c0);
-          m0 = fmaxf(m0, x.x);
-          m1 = fmaxf(m1, x.y);
-        }
-      float l0 = 0.0f, l1 = 0.0f;
+      float m0 = kNeg, m1 = kNeg, l0 = 0.0f, l1 = 0.0f;
       float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int p = p0; p < p1; p++)
-        if (info[p].unit >= 0) {
-          const float* q = piece(p);
-          const float2 x = *reinterpret_cast<const float2*>(q + c0);
-          const float2 l = *reinterpret_cast<const float2*>(q + 8 * NT + c0);
-          const float4 z = *reinterpret_cast<const float4*>(q + 16 * NT + (f * 32 + lane) * 4);
-          const float e0 = ex2(x.x - m0), e1 = ex2(x.y - m1);
-          l0 = fmaf(e0, l.x, l0);
-          l1 = fmaf(e1, l.y, l1);
-          o.x = fmaf(e0, z.x, o.x);
-          o.y = fmaf(e1, z.y, o.y);
-          o.z = fmaf(e0, z.z, o.z);
-          o.w = fmaf(e1, z.w, o.w);
+      for (unsigned todo = chain; todo;) {
+        float2 x[4], l[4];
+        float4 z[4];
+        float n0 = m0, n1 = m1;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float* q = piece(todo ? __ffs(todo) - 1 : p0);
+          const bool there = todo != 0;
+          todo &= todo - 1;
+          n += there;
+          x[i] = *reinterpret_cast<const float2*>(q + c0);
+          l[i] = *reinterpret_cast<const float2*>(q + 8 * NT + c0);
+          z[i] = *reinterpret_cast<const float4*>(q + 16 * NT + (f * 32 + lane) * 4);
+          if (there) {
+            n0 = fmaxf(n0, x[i].x);
+            n1 = fmaxf(n1, x[i].y);
+          }
         }
+        const float r0 = ex2(m0 - n0), r1 = ex2(m1 - n1);
+        m0 = n0;
+        m1 = n1;
+        l0 *= r0;
+        l1 *= r1;
+        o = make_float4(o.x * r0, o.y * r1, o.z * r0, o.w * r1);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          if (i >= n) break;
+          const float e0 = ex2(x[i].x - m0), e1 = ex2(x[i].y - m1);
+          l0 = fmaf(e0, l[i].x, l0);
+          l1 = fmaf(e1, l[i].y, l1);
+          o.x = fmaf(e0, z[i].x, o.x);
+          o.y = fmaf(e1, z[i].y, o.y);
+          o.z = fmaf(e0, z[i].z, o.z);
+          o.w = fmaf(e1, z[i].w, o.w);
+        }
+      }
       if (whole) {
         const float i0 = l0 != 0.0f ? 1.0f / l0 : 0.0f, i1 = l1 != 0.0f ? 1.0f / l1 : 0.0f;
-        const int d = frag_d<BITS, D, GS>(f / NT, g), h = first.unit % v.Hkv;
+        const int d = frag_d<BITS, D, GS>(f / NT, g), h = unit % v.Hkv;
         store_out<NT, BF>(a, k, h, c0, d, o.x * i0, o.z * i0);
         store_out<NT, BF>(a, k, h, c0 + 1, d, o.y * i1, o.w * i1);
       } else {
@@ -973,16 +989,11 @@ __global__ void __launch_bounds__(Cfg<BITS, D, GS, NT, ST>::W * 32, 1)
       }
     }
     if (!whole) {
-      if (flags & 1) slot1 = first.unit;
-      else slot0 = (flags & 2) ? 2 : 1;
+      if (flags & 1) mt = make_int4(unit, mt.y | (k.cols << 8), k.row0, k.col0);
+      else mt.y |= (flags & 2) ? 2 : 1;
     }
-    p0 = p1;
   }
-  if (tid == 0) {
-    Block k{};
-    if (slot1 >= 0) k = get_block<NC>(a, P, slot1 / v.Hkv);
-    ws.meta[blockIdx.x] = make_int4(slot1, slot0 | (k.cols << 8), k.row0, k.col0);
-  }
+  if (tid == 0) ws.meta[blockIdx.x] = mt;
 }
 
 // Block (c, f): the unit that begins in CTA c and goes on, fragment f; its
@@ -1000,12 +1011,18 @@ __global__ void __launch_bounds__(kMergeWarps * 32) cols_merge_kernel(const Attn
   const View& v = a.v;
   const int c = blockIdx.x, n = gridDim.x, f = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int unit = ws.meta[c].x;
+  const int4 where = ws.meta[c];
+  int end = n - 1;  // the CTA that ends the unit: the first after c that ends one
+  for (int i = c + 1 + tid; i < n; i += kMergeWarps * 32)
+    if ((ws.meta[i].y & 255) == 2) {
+      end = i;
+      break;
+    }
+  const int unit = where.x;
   if (unit < 0) return;
   if (tid == 0) s_end = n - 1;
   __syncthreads();
-  for (int i = c + 1 + tid; i < n; i += kMergeWarps * 32)
-    if ((ws.meta[i].y & 255) == 2) atomicMin(&s_end, i);
+  if (end < n - 1) atomicMin(&s_end, end);
   __syncthreads();
   const int last = s_end;
   auto piece = [&](int i) -> const float* {
@@ -1052,7 +1069,6 @@ __global__ void __launch_bounds__(kMergeWarps * 32) cols_merge_kernel(const Attn
     o.w = fmaf(e1, z.w, o.w);
   }
   const float i0 = l0 != 0.0f ? 1.0f / l0 : 0.0f, i1 = l1 != 0.0f ? 1.0f / l1 : 0.0f;
-  const int4 where = ws.meta[c];
   Block k;
   k.cols = where.y >> 8;
   k.row0 = where.z;
