@@ -4,18 +4,18 @@
 //
 // A unit is one (sequence, kv head) and MR query rows (row c is token c / rep,
 // head c % rep: every query head of the group shares the tile's K and V).  Its
-// 128-key tiles are dequantized once, to the dtype, into 128-byte-swizzled
+// 128-key tiles (D 256: 64) are dequantized once, to the dtype, into 128-byte-swizzled
 // shared tiles and serve all MR rows: S = Q K^T into TMEM, softmax from TMEM
 // to P in the same columns, O += P V with A from TMEM.
 //   * D 64 / 128: MR 256, two row tiles of 128 (TMEM lanes) in turn: the tensor
 //     core works on one while the softmax warps have the other.
 //   * D 256: MR 128 (its O takes 256 TMEM columns), two S buffers instead.
-// Warps: 8 per row tile for the softmax (two threads share a row, 64 keys each;
+// Warps: 8 per row tile for the softmax (two threads share a row, half of the keys each;
 // one exchange of the maximum per tile), 7 that dequantize (a thread owns a key
 // row of K or of V; the 32-row blocks K 0-3, V 0-3 of each tile go round), 1
 // that issues the MMAs.  All hand-offs are mbarriers with bounded waits.  A wait
-// tells two neighbouring phases apart only, so a barrier whose waiter may be two
-// releases behind comes in two, taken alternately.
+// tells two neighbouring phases apart only, so a barrier whose waiter may be more
+// releases behind comes in several, taken in turn.
 //
 // Roundings: K, V (as a dense cache of the dtype holds them) and the
 // probabilities go through the tensor core in the dtype; logits, statistics
@@ -40,15 +40,18 @@ template <int BITS, int D, int GS>
 struct Chunk {
   static constexpr int QT = D == 256 ? 1 : 2;   // row tiles of 128
   static constexpr int MR = 128 * QT;
-  static constexpr int KT = 128;                // keys per tile
-  static constexpr int KB = D == 256 ? 1 : 2;   // K (and V) buffers
-  static constexpr int PANEL = 128 * 128;       // bytes: 128 rows of 64 elements
-  static constexpr int TILE = D / 64 * PANEL;   // bytes of a Q, K or V tile
+  static constexpr int KL = D == 256 ? 6 : 7, KT = 1 << KL;  // keys per tile: 64 or 128
+  static constexpr int NBK = KT / 32, BL = KL - 4;  // 32-row blocks of K; log2 of K's and V's
+  static constexpr int KB = 2;                  // K (and V) buffers
+  static constexpr int QPANEL = 128 * 128;      // bytes: 128 rows of 64 elements
+  static constexpr int QTILE = D / 64 * QPANEL;
+  static constexpr int PANEL = KT * 128;        // the same of a K or V tile
+  static constexpr int TILE = D / 64 * PANEL;
   static constexpr int CRB = D * BITS / 8;
   static constexpr int PRB = D / GS * 4;
   static constexpr int HALF = kTileRows * (CRB + PRB);
   static constexpr int O_Q = 0;
-  static constexpr int O_K = QT * TILE;
+  static constexpr int O_K = QT * QTILE;
   static constexpr int O_V = O_K + KB * TILE;
   static constexpr int O_PLAN = O_V + KB * TILE;
   static constexpr int O_TMP = (O_PLAN + (kPlanMax + 1) * 12 + 4 + 15) / 16 * 16;
@@ -68,7 +71,7 @@ struct Chunk {
 
 struct ChunkBars {
   uint64_t q_full[2], s_full[2], p_full[2], o_done[2];
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t k_full[2], v_full[2], k_empty[4], v_empty[4];
   uint64_t x[2][4][2];  // the exchange of two warps with the same rows, alternating
 };
 
@@ -93,7 +96,7 @@ struct Walk {
       else y = mid;
     }
     gi = x;
-    k = get_block<C::MR, 7>(a, P, gi);
+    k = get_block<C::MR, C::KL>(a, P, gi);
     const long long rel = t0 - P.tpre[gi] * Hkv;
     h = (int)(rel / k.nt);
     i0 = (int)(rel - (long long)h * k.nt);
@@ -108,7 +111,7 @@ struct Walk {
       do {
         gi++;
       } while (P.tpre[gi + 1] == P.tpre[gi]);
-      k = get_block<C::MR, 7>(a, P, gi);
+      k = get_block<C::MR, C::KL>(a, P, gi);
     }
     i0 = 0;
     i1 = (int)min((long long)k.nt, left);
@@ -250,10 +253,12 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       attn::mbar_init(&bar.s_full[i], 1);
       attn::mbar_init(&bar.p_full[i], 256);
       attn::mbar_init(&bar.o_done[i], 1);
-      attn::mbar_init(&bar.k_full[i], 128);
+      attn::mbar_init(&bar.k_full[i], C::KT);
+      attn::mbar_init(&bar.v_full[i], C::KT);
       attn::mbar_init(&bar.k_empty[i], 1);
-      attn::mbar_init(&bar.v_full[i], 128);
+      attn::mbar_init(&bar.k_empty[i + 2], 1);
       attn::mbar_init(&bar.v_empty[i], 1);
+      attn::mbar_init(&bar.v_empty[i + 2], 1);
       for (int w = 0; w < 8; w++) attn::mbar_init(&bar.x[w >> 2][w & 3][i], 64);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -272,7 +277,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
   } else {
     long long* tpre = reinterpret_cast<long long*>(sm + C::O_PLAN);
     int* gpre = reinterpret_cast<int*>(tpre + kPlanMax + 1);
-    const int NG_ = build_plan<C::MR, 7>(a, gpre, tpre, ws.max_blocks,
+    const int NG_ = build_plan<C::MR, C::KL>(a, gpre, tpre, ws.max_blocks,
                                          reinterpret_cast<long long*>(sm + C::O_TMP), blockIdx.x == 0);
     P = Plan{gpre, tpre, NG_};
   }
@@ -287,7 +292,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
   // column blocks that see no key: zero rows
   for (long long gi = c; gi < P.NG; gi += gridDim.x) {
     if (P.tpre[gi + 1] != P.tpre[gi]) continue;
-    const Block k = get_block<C::MR, 7>(a, P, (int)gi);
+    const Block k = get_block<C::MR, C::KL>(a, P, (int)gi);
     for (int64_t e = tid; e < (int64_t)v.Hkv * k.cols * (D / 2); e += C::kThreads) {
       const int d = (int)(e % (D / 2)) * 2, x = (int)(e / (D / 2));
       store_out<1, BF>(a, k, x / k.cols, x % k.cols, d, 0.0f, 0.0f);
@@ -301,7 +306,8 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
     return false;
   };
   if (warp < C::kSoftWarps) {
-    // ------------------------------------- softmax: half a row (64 keys) a thread
+    // --------------------------------- softmax: half of a row's keys a thread
+    constexpr int VW = C::KT / 64;  // 32-key words of a half
     const int q = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     // in shared memory, to spare registers
@@ -339,7 +345,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       const int col = k.col0 + (live ? row : 0), tok = col / a.rep;
       const int head = w_.h * a.rep + (col - tok * a.rep);
       const uint16_t* src = a.q + (int64_t)(k.row0 + tok) * a.q_row + (int64_t)head * a.q_head;
-      uint8_t* dst = sm + C::O_Q + q * C::TILE;
+      uint8_t* dst = sm + C::O_Q + q * C::QTILE;
 #pragma unroll 4
       for (int e = half * (D / 16); e < (half + 1) * (D / 16); e++) {
         uint16_t x[8];
@@ -359,7 +365,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
           const uint32_t hi = x[BITS == 4 ? nib_pos(2 * i + 1) : 2 * i + 1];
           w[i] = live ? (lo | (hi << 16)) ^ flip : 0u;
         }
-        *reinterpret_cast<uint4*>(dst + (e >> 3) * C::PANEL + sw128(r, (e & 7) * 8)) =
+        *reinterpret_cast<uint4*>(dst + (e >> 3) * C::QPANEL + sw128(r, (e & 7) * 8)) =
             make_uint4(w[0], w[1], w[2], w[3]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -382,34 +388,35 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       const int i1 = wk.i1;
       for (int i = wk.i0; i < i1; i++, tc++) {
         const int sb = QT == 2 ? q : tc & 1;
-        const uint32_t tS = tm + lanes + sb * 128 + half * 64;  // its 64 keys' columns
+        const uint32_t tS = tm + lanes + sb * 128 + half * (C::KT / 2);  // its keys' columns
         if (!wait_all(&bar.s_full[sb], QT == 2 ? tc & 1 : (tc >> 1) & 1)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const int kb = (tile_of(k, i) << 7) + half * 64;
-        const uint32_t bad2 =
-            *reinterpret_cast<volatile uint16_t*>(const_cast<uint8_t*>(s_bad) + (tc & 3) * 4 + half * 2);
-        const bool full = kb + 63 <= k.pmin && bad2 == 0 &&
-                          (a.window == 0 || kb > k.pmax - a.window || kb + 63 < a.sinks);
-        uint32_t vis[2];
+        const int kb = (tile_of(k, i) << C::KL) + half * (C::KT / 2);
+        // two bits for each 32 keys: 16-key tiles without a page
+        uint32_t bad2 = s_bad[(tc & 3) * 4 + half * VW];
+        if (VW == 2) bad2 |= (uint32_t)s_bad[(tc & 3) * 4 + half * VW + 1] << 8;
+        const bool full = kb + C::KT / 2 - 1 <= k.pmin && bad2 == 0 &&
+                          (a.window == 0 || kb > k.pmax - a.window || kb + C::KT / 2 - 1 < a.sinks);
+        uint32_t vis[VW];
         if (!full) {
           // bits of the keys that this row sees
 #pragma unroll
-          for (int w = 0; w < 2; w++) {
+          for (int w = 0; w < VW; w++) {
             const int j0 = kb + 32 * w;
             auto upto = [](int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); };
             uint32_t x = upto(p + 1 - j0);
             if (a.window > 0) x &= ~upto(p - a.window + 1 - j0) | upto(a.sinks - j0);
-            const uint32_t b2 = (bad2 >> (8 * w)) & 3u;  // two 16-key tiles without a page
+            const uint32_t b2 = (bad2 >> (8 * w)) & 3u;
             x &= ~(((b2 & 1u) ? 0x0000ffffu : 0u) | ((b2 & 2u) ? 0xffff0000u : 0u));
             vis[w] = x;
           }
         }
         float mx = kNeg;
 #pragma unroll
-        for (int w = 0; w < 2; w++) {
+        for (int w = 0; w < VW; w++) {
           uint32_t s[32];
           tmem_ld32(tS + 32 * w, s);
           tmem_wait_ld();
@@ -457,7 +464,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         const float2 cc = make_float2(c2, c2), mm = make_float2(-m, -m);
         float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int w = 0; w < 2; w++) {
+        for (int w = 0; w < VW; w++) {
           uint32_t s[32], pk[16];
           tmem_ld32(tS + 32 * w, s);
           tmem_wait_ld();
@@ -563,25 +570,25 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
     const int total = (int)(t1 - t0);
     // where block n's row lies: list index of its tile, position, page
     auto seek = [&](int n) {
-      while ((n >> 3) - first >= wk.i1 - wk.i0) {
+      while ((n >> C::BL) - first >= wk.i1 - wk.i0) {
         first += wk.i1 - wk.i0;
         wk.next(a);
       }
     };
-    auto key_of = [&](int n) { return (tile_of(wk.k, wk.i0 + (n >> 3) - first) << 7) + (n & 3) * 32 + lane; };
+    auto key_of = [&](int n) { return (tile_of(wk.k, wk.i0 + (n >> C::BL) - first) << C::KL) + (n & (C::NBK - 1)) * 32 + lane; };
     auto page_of = [&](int j) -> int {  // -1: nobody sees the row
       if ((j >> 4) > (wk.k.pmax >> 4)) return -1;
       return __ldg(v.table + (int64_t)wk.k.b * v.table_stride + (j >> v.page_shift));
     };
     int n = warp - C::kSoftWarps, j = 0, page = -1;
-    if (n < 8 * total) {
+    if (n < total << C::BL) {
       seek(n);
       j = key_of(n);
       page = page_of(j);
     }
-    while (n < 8 * total) {
-      const int tc = n >> 3, quarter = n & 3;
-      const bool is_v = n & 4;
+    while (n < total << C::BL) {
+      const int tc = n >> C::BL, quarter = n & (C::NBK - 1);
+      const bool is_v = n & C::NBK;
       const Block& k = wk.k;
       const int klo = a.window > 0 ? max(0, k.pmin - a.window + 1) : 0;
       const bool wanted = j <= k.pmax && (j >= klo || j < a.sinks);
@@ -608,17 +615,17 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       const unsigned lost = __ballot_sync(0xffffffffu, here && wanted && !found);
       // the next block's page, on its way while this one is converted
       n += C::kDequantWarps;
-      if (n < 8 * total) {
+      if (n < total << C::BL) {
         seek(n);
         j = key_of(n);
         page = page_of(j);
       }
       const int buf = KB == 2 ? tc & 1 : 0;
-      // the buffer's last reader was tile tc - KB.  The barriers go by the parity
-      // of that tile even with one buffer: a warp that had no V block for some
-      // tiles may be two releases behind, which one barrier's parity cannot tell.
+      // the buffer's last reader was tile tc - KB.  Four barriers by that tile's
+      // number: a warp that had no V block for some tiles may be several releases
+      // behind, which fewer barriers' parities cannot tell apart.
       const int was = tc - KB;
-      if (was >= 0 && !wait_all(is_v ? &bar.v_empty[was & 1] : &bar.k_empty[was & 1], (was >> 1) & 1)) break;
+      if (was >= 0 && !wait_all(is_v ? &bar.v_empty[was & 3] : &bar.k_empty[was & 3], (was >> 2) & 1)) break;
       const int r = quarter * 32 + lane;
       uint8_t* dst = sm + (is_v ? C::O_V : C::O_K) + buf * C::TILE + (r >> 3) * 1024 + (r & 7) * 128;
 #pragma unroll
@@ -651,8 +658,8 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       if (!elect_one()) return;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ks++) {
-        const uint32_t off = (ks >> 2) * C::PANEL + 32 * (ks & 3);
-        umma_ss_lo(dS, dq0 + ((q * C::TILE + off) >> 4), dk0 + ((buf * C::TILE + off) >> 4), iqk, ks ? 1u : 0u);
+        const uint32_t oq = (ks >> 2) * C::QPANEL + 32 * (ks & 3), ok_ = (ks >> 2) * C::PANEL + 32 * (ks & 3);
+        umma_ss_lo(dS, dq0 + ((q * C::QTILE + oq) >> 4), dk0 + ((buf * C::TILE + ok_) >> 4), iqk, ks ? 1u : 0u);
       }
       umma_commit(&bar.s_full[QT == 2 ? q : t & 1]);
     };
@@ -662,7 +669,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       if (!elect_one()) return;
 #pragma unroll
       for (int ks = 0; ks < C::KT / 16; ks++)
-        umma_ts_lo(tm + C::TM_O + q * D, tP + 8 * (ks & 3) + 64 * (ks >> 2), dv0 + ((buf * C::TILE + 2048 * ks) >> 4), ipv,
+        umma_ts_lo(tm + C::TM_O + q * D, tP + 8 * (ks % (C::KT / 32)) + C::KT / 2 * (ks / (C::KT / 32)), dv0 + ((buf * C::TILE + 2048 * ks) >> 4), ipv,
                 (first && ks == 0) ? 0u : 1u);
       umma_commit(&bar.o_done[QT == 2 ? q : t & 1]);
     };
@@ -678,7 +685,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         if (!wait_all(&bar.q_full[q], u & 1)) return false;
       tc_fence_after();
       for (int q = 0; q < QT; q++) qk(q, t);
-      commit(&bar.k_empty[t & 1]);
+      commit(&bar.k_empty[t & 3]);
       return true;
     };
     const int total = (int)(t1 - t0);
@@ -697,23 +704,23 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         if (!(ok = wait_all(&bar.p_full[1], tc & 1))) break;
         tc_fence_after();
         pv(1, tc, first);
-        commit(&bar.v_empty[tc & 1]);
+        commit(&bar.v_empty[tc & 3]);
         if (more) {
           qk(1, tc + 1);
-          commit(&bar.k_empty[(tc + 1) & 1]);
+          commit(&bar.k_empty[(tc + 1) & 3]);
         }
       } else {
         if (more) {
           if (!(ok = kwait(tc + 1))) break;
           tc_fence_after();
           qk(0, tc + 1);
-          commit(&bar.k_empty[(tc + 1) & 1]);
+          commit(&bar.k_empty[(tc + 1) & 3]);
         }
         ok = vwait(tc) && wait_all(&bar.p_full[tc & 1], (tc >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
         pv(0, tc, first);
-        commit(&bar.v_empty[tc & 1]);
+        commit(&bar.v_empty[tc & 3]);
       }
       if (!more && tc + 1 < total) ok = kwait(tc + 1) && start(tc + 1, ++u);
     }
@@ -791,7 +798,7 @@ int32_t launch_chunk_one(const AttnArgs& a, const Work& ws, int ctas, int dev, c
   int32_t rc = kernel_setup(reinterpret_cast<const void*>(kern), C::kThreads, C::SMEM, dev, nullptr);
   if (rc) return rc;
   if ((rc = kernel_carveout(reinterpret_cast<const void*>(merge), dev))) return rc;
-  if (ws.tpre) KVQ_CUDA_TRY(launch_pdl(plan_kernel<C::MR, 7>, dim3(1), dim3(1024), 0, st, a, ws));
+  if (ws.tpre) KVQ_CUDA_TRY(launch_pdl(plan_kernel<C::MR, C::KL>, dim3(1), dim3(1024), 0, st, a, ws));
   KVQ_CUDA_TRY(launch_pdl(kern, dim3((unsigned)ctas), dim3(C::kThreads), C::SMEM, st, a, ws));
   KVQ_CUDA_TRY(launch_pdl(merge, dim3((unsigned)ctas, C::MR / 32), dim3(256), 0, st, a, ws));
   return KVQ_OK;
