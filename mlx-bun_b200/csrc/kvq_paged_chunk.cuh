@@ -166,9 +166,11 @@ struct Dequant {
         const uint32_t u = w[i >> 1];
         if constexpr (BF) {
           // codes up to 255 have no bf16 form with a free offset: f32, rounded once
-          const float a = __uint_as_float(prmt(u, 0x4b000000u, (i & 1) ? 0x7442u : 0x7440u)) - 8388608.0f;
-          const float b = __uint_as_float(prmt(u, 0x4b000000u, (i & 1) ? 0x7443u : 0x7441u)) - 8388608.0f;
-          const __nv_bfloat162 t = __floats2bfloat162_rn(fmaf(a, sf, zf), fmaf(b, sf, zf));
+          float2 x = make_float2(__uint_as_float(prmt(u, 0x4b000000u, (i & 1) ? 0x7442u : 0x7440u)),
+                                 __uint_as_float(prmt(u, 0x4b000000u, (i & 1) ? 0x7443u : 0x7441u)));
+          x = __fadd2_rn(x, make_float2(-8388608.0f, -8388608.0f));  // from 2^23 + c
+          x = __ffma2_rn(x, make_float2(sf, sf), make_float2(zf, zf));
+          const __nv_bfloat162 t = __floats2bfloat162_rn(x.x, x.y);
           r[i] = *reinterpret_cast<const uint32_t*>(&t);
         } else {
           const uint32_t x = prmt(u, 0x64646464u, (i & 1) ? 0x4342u : 0x4140u);
