@@ -12,7 +12,7 @@
 //   * D 256: MR 128 (its O takes 256 TMEM columns), two S buffers instead.
 // Warps: 8 per row tile for the softmax (two threads share a row, half of the keys each;
 // one exchange of the maximum per tile), 7 that dequantize (a thread owns a key
-// row of K or of V; the 32-row blocks K 0-3, V 0-3 of each tile go round), 1
+// row of K or of V; the 32-row blocks of K and V of each tile go round), 1
 // that issues the MMAs.  All hand-offs are mbarriers with bounded waits.  A wait
 // tells two neighbouring phases apart only, so a barrier whose waiter may be more
 // releases behind comes in several, taken in turn.
@@ -29,7 +29,9 @@
 // the pieces of a cut unit (m, l, O in f32) meet in the merge kernel in order.
 //
 // Measured (B200): 512 rows over 16,896 keys, 32 query and 8 kv heads, D 128, 8
-// bits (139.6 GFLOP): 178 us, 783 TFLOP/s, about 5,000 clocks a tile.
+// bits (139.6 GFLOP): 181 us, 771 TFLOP/s, about 5,000 clocks a tile.  D 256, two
+// chunks of up to 1,024 rows, window 1,024, 8 bits: 110 us; one K / V buffer of 128
+// keys instead of two of 64 took 133.
 #include "kvq_paged_cols.cuh"
 #include "kvq_tc.cuh"
 
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       p = p_next;
     }
   } else if (warp < C::kMmaWarp) {
-    // ------------------------- dequantize: 32-row blocks K 0-3, V 0-3 of each tile
+    // ------------------------- dequantize: 32-row blocks of K, then of V, of each tile
     constexpr int RW = C::CRB / 16;  // 16-byte words of a code row
     Walk<BITS, D, GS> wk;
     wk.start(a, P, t0, t1);
