@@ -5,7 +5,8 @@ quantized format (kvq_paged, include/kvq.h).  Which pages a sequence owns is
 the caller's page table; lengths and row offsets are device arrays, so a CUDA
 graph of ``append`` + ``sdpa_decode`` serves every later step.  The same
 (page_table, seq_lens, cu_rows) describe a step to all calls: ``seq_lens``
-counts each sequence's tokens with the step's rows included.
+counts each sequence's tokens with the step's rows included.  Rows of
+``page_table`` may share pages but not memory (a broadcast row is refused).
 """
 from __future__ import annotations
 
@@ -128,7 +129,7 @@ class PagedQuantizedKVCache:
                     cu_rows.get_device() != dev or not cu_rows.is_contiguous():
                 raise ValueError("cu_rows must be contiguous int32 [batch + 1] on the cache's device")
             cu = cu_rows.data_ptr()
-        return _lib.PagedBatch(page_table.data_ptr(), max(page_table.stride(0), pages[1]),
+        return _lib.PagedBatch(page_table.data_ptr(), page_table.stride(0),
                                seq_lens.data_ptr(), cu, B, pages[1], rows)
 
     def _rows(self, x: torch.Tensor, name: str, heads: int | None = None):

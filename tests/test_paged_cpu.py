@@ -125,3 +125,21 @@ def test_python_refusals():
     with pytest.raises(kvq.KvqError):
         kvq.PagedQuantizedKVCache.pool_shape(2, 24, 2, 64, 32, 4, torch.float16)
     assert kvq.PagedQuantizedKVCache.pool_shape(3, 32, 2, 128, 64, 4) == (3, 2, 2, 576)
+
+
+def test_overlapping_table_rows_are_refused():
+    # a table that one row is broadcast into has the row stride 0: its rows
+    # must not be taken for max_pages apart, behind the end of its memory
+    import kvq
+    cache = object.__new__(kvq.PagedQuantizedKVCache)
+    cache._index = -1  # the device index of CPU tensors; no launch follows
+    lens = torch.zeros(3, dtype=torch.int32)
+    for table, stride in ((torch.zeros(1, 8, dtype=torch.int32).expand(3, 8), 0),
+                          (torch.zeros(16, dtype=torch.int32).as_strided((3, 8), (4, 1)), 4),
+                          (torch.zeros(1, 1, dtype=torch.int32).expand(3, 1), 0)):
+        b = cache._batch(3, table, lens, None)
+        assert b.table_stride == stride
+        assert sdpa(paged(), b, decode=True) != 0 and "table_stride" in error()
+        assert append(paged(), b) != 0 and "table_stride" in error()
+    b = cache._batch(3, torch.zeros(3, 24, dtype=torch.int32)[:, :8], lens, None)
+    assert (b.table_stride, b.max_pages) == (24, 8)
