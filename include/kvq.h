@@ -477,8 +477,8 @@ int32_t kvq_paged_append(const kvq_paged* cache, const kvq_paged_batch* batch, c
 
 /* Causal attention of the step's query rows over their sequences' pages.
  * q: device [rows, q_heads, head_dim] with element strides (row, head); out:
- * contiguous [rows, q_heads, head_dim]; query head h uses kv head h / (q_heads
- * / kv_heads).  A query at position p sees key j when j <= p and (window == 0
+ * contiguous [rows, q_heads, head_dim], at any element of its buffer; query
+ * head h uses kv head h / (q_heads / kv_heads).  A query at position p sees key j when j <= p and (window == 0
  * or j > p - window or j < sinks): a sliding window with the first `sinks`
  * tokens kept visible.  A row that sees no key gives zeros.  k and v are code
  * * scale + bias, logits and softmax are f32, the output is rounded once.

@@ -78,6 +78,7 @@ struct AttnArgs {
   const uint16_t* q;
   int64_t q_row, q_head;
   uint16_t* out;
+  int out_align;  // rows start at 16-byte (2), 4-byte (1) or element (0) borders
   int Hq, rep;
   float scale;
   int window, sinks;

@@ -108,6 +108,8 @@ int32_t sdpa(const kvq_paged* c, const kvq_paged_batch* b, bool decode, const vo
   a.q_row = q_strides[0];
   a.q_head = q_strides[1];
   a.out = static_cast<uint16_t*>(out);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(out);
+  a.out_align = at % 16 == 0 ? 2 : at % 4 == 0 ? 1 : 0;  // head_dim elements are a multiple of 16 bytes
   a.scale = scale;
   a.window = window;
   a.sinks = window > 0 ? sinks : 0;

@@ -552,7 +552,15 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
               for (int i = 0; i < 4; i++)
                 w[i] = (uint32_t)attn::f_to_dt<BF>(x[e + 2 * i] * inv) |
                        ((uint32_t)attn::f_to_dt<BF>(x[e + 2 * i + 1] * inv) << 16);
-              *reinterpret_cast<uint4*>(dst + d + e) = make_uint4(w[0], w[1], w[2], w[3]);
+              if (a.out_align == 2) {
+                *reinterpret_cast<uint4*>(dst + d + e) = make_uint4(w[0], w[1], w[2], w[3]);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                  dst[d + e + 2 * i] = (uint16_t)w[i];
+                  dst[d + e + 2 * i + 1] = (uint16_t)(w[i] >> 16);
+                }
+              }
             }
           }
         } else {

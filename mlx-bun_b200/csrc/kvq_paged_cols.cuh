@@ -619,8 +619,13 @@ __device__ __forceinline__ void store_out(const AttnArgs& a, const Block& k, int
   if (c >= k.cols) return;
   const int col = k.col0 + c, tok = col / a.rep, hh = col - tok * a.rep;
   uint16_t* dst = a.out + ((int64_t)(k.row0 + tok) * a.Hq + h * a.rep + hh) * a.v.D + d;
-  *reinterpret_cast<uint32_t*>(dst) =
-      (uint32_t)attn::f_to_dt<BF>(x) | ((uint32_t)attn::f_to_dt<BF>(y) << 16);
+  const uint16_t lo = attn::f_to_dt<BF>(x), hi = attn::f_to_dt<BF>(y);
+  if (a.out_align) {
+    *reinterpret_cast<uint32_t*>(dst) = (uint32_t)lo | ((uint32_t)hi << 16);
+  } else {  // a view that starts at an odd element
+    dst[0] = lo;
+    dst[1] = hi;
+  }
 }
 
 // Close a segment: sums over the lanes of a column, outputs in natural units,

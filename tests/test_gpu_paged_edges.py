@@ -1,0 +1,76 @@
+"""Calls of the paged cache at the edges of what its documentation allows, on
+the GPU against the plain 64-bit implementation of tests/paged_ref.py."""
+import numpy as np
+import pytest
+import torch
+
+import paged_ref as R
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def _kvq():
+    import kvq
+    return kvq
+
+
+def _cache(ref):
+    kvq = _kvq()
+    return kvq.PagedQuantizedKVCache(ref.pool.shape[0], ref.page, ref.heads, ref.d, ref.gs,
+                                     ref.bits, ref.dt, pool=ref.pool.cuda())
+
+
+def _cu(rows):
+    return [0] + list(np.cumsum(rows))
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _pages(lens, page):
+    return sum(-(-max(n, 0) // page) for n in lens) + 3
+
+
+# --------------------------------------------------------- where out begins --
+
+OUT = [
+    # dt, bits, gs, Hq, Hkv, D, page, lens, rows (None: decode)
+    (F16, 4, 64, 8, 2, 128, 16, [1000, 1, 17], None),     # 4 columns a block
+    (BF16, 8, 64, 16, 2, 64, 32, [700, 0, 90], None),     # 8
+    (F16, 8, 32, 16, 1, 128, 16, [300], None),            # 16
+    (F16, 4, 64, 8, 2, 128, 16, [100, 40], [6, 3]),       # drafts
+    (BF16, 4, 64, 8, 2, 128, 16, [700, 300], [257, 300]),
+    (F16, 8, 64, 4, 2, 256, 32, [400, 130], [130, 100]),
+    (BF16, 8, 64, 16, 8, 256, 32, [2000, 1500], [600, 500]),  # units held whole and cut
+]
+
+
+@pytest.mark.parametrize("case", OUT, ids=lambda c: "-".join(str(x) for x in c[1:]))
+@pytest.mark.parametrize("cut", [1, 2, 3, 4])
+def test_out_may_start_at_any_element(case, cut):
+    """The same bits wherever a contiguous `out` starts in its buffer, and
+    nothing written beside it."""
+    dt, bits, gs, hq, hkv, d, page, lens, rows = case
+    gen = torch.Generator().manual_seed(31)
+    ref = R.random_pool(gen, _pages(lens, page), page, hkv, d, gs, bits, dt)
+    table = R.make_table(gen, lens, page, ref.pool.shape[0]).cuda()
+    cache = _cache(ref)
+    n = len(lens) if rows is None else sum(rows)
+    q = torch.randn(n, hq, d, generator=gen).to(dt).cuda()
+
+    def call(out):
+        if rows is None:
+            return cache.sdpa_decode(q, table, _i32(lens), 0.1, out=out)
+        return cache.sdpa_prefill(q, table, _i32(lens), _i32(_cu(rows)), 0.1, out=out)
+
+    want = call(torch.zeros(n, hq, d, dtype=dt, device="cuda"))
+    buf = torch.full((n * hq * d + 8,), 7.0, dtype=dt, device="cuda")
+    out = buf[cut:cut + n * hq * d].view(n, hq, d)
+    assert out.data_ptr() % 16 == 2 * cut
+    assert call(out) is out
+    cache.check()
+    assert torch.equal(out.view(torch.int16), want.view(torch.int16))
+    assert (buf[:cut] == 7.0).all() and (buf[cut + n * hq * d:] == 7.0).all()
