@@ -11,6 +11,10 @@ using namespace kvq;
 
 namespace {
 
+// Every device array starts at a multiple of its elements' size (a null one
+// does): the kernels load whole elements.
+bool aligned(const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
+
 int32_t make_view(const kvq_paged* c, const kvq_paged_batch* b, paged::View& v) {
   if (!c || !b) return fail(KVQ_ERR_ARG, "paged: NULL cache / batch");
   if (!c->pool || !c->status) return fail(KVQ_ERR_ARG, "paged: NULL pool / status");
@@ -29,6 +33,8 @@ int32_t make_view(const kvq_paged* c, const kvq_paged_batch* b, paged::View& v) 
   if (b->batch < 0 || b->rows < 0 || b->max_pages < 0) return fail(KVQ_ERR_ARG, "paged: batch, rows and max_pages must be >= 0");
   if (b->batch > 0 && (!b->seq_lens || (b->max_pages > 0 && !b->page_table)))
     return fail(KVQ_ERR_ARG, "paged: NULL page_table / seq_lens");
+  if (!aligned(c->status, 4) || !aligned(b->page_table, 4) || !aligned(b->seq_lens, 4) || !aligned(b->cu_rows, 4))
+    return fail(KVQ_ERR_ARG, "paged: status, page_table, seq_lens and cu_rows must be 4-byte aligned");
   if (b->table_stride < b->max_pages && b->batch > 1) return fail(KVQ_ERR_ARG, "paged: table_stride smaller than max_pages");
   if (((int64_t)b->max_pages << shift) > 0x7fffffff) return fail(KVQ_ERR_ARG, "paged: max_pages * page_size passes 2^31");
   v = paged::View{};
@@ -104,6 +110,7 @@ int32_t sdpa(const kvq_paged* c, const kvq_paged_batch* b, bool decode, const vo
   if ((int64_t)window >= ((int64_t)a.v.max_pages << a.v.page_shift)) window = 0;
   if (a.v.rows == 0 || a.v.B == 0) return KVQ_OK;
   if (!q || !q_strides || !out) return fail(KVQ_ERR_ARG, "paged: NULL q / q_strides / out");
+  if (!aligned(q, 2) || !aligned(out, 2)) return fail(KVQ_ERR_ARG, "paged: q and out must be 2-byte aligned");
   a.q = static_cast<const uint16_t*>(q);
   a.q_row = q_strides[0];
   a.q_head = q_strides[1];
@@ -189,6 +196,7 @@ int32_t kvq_paged_append(const kvq_paged* c, const kvq_paged_batch* b, const voi
         return fail(KVQ_ERR_ARG, "paged: rope dims must be even and within head_dim");
       if (rope->dims > 0 && !rope->freqs && !(rope->base > 0.0f))
         return fail(KVQ_ERR_ARG, "paged: rope base must be positive (or freqs given)");
+      if (!aligned(rope->freqs, 4)) return fail(KVQ_ERR_ARG, "paged: rope freqs must be 4-byte aligned");
       a.rope.dims = rope->dims;
       a.rope.half = rope->dims / 2;
       a.rope.traditional = rope->traditional != 0;
@@ -199,6 +207,8 @@ int32_t kvq_paged_append(const kvq_paged* c, const kvq_paged_batch* b, const voi
     }
     if (a.v.rows == 0 || a.v.B == 0) return KVQ_OK;
     if (!k || !v || !k_strides || !v_strides) return fail(KVQ_ERR_ARG, "paged: NULL k / v / strides");
+    if (!aligned(k, 2) || !aligned(v, 2) || (q && (!aligned(q, 2) || !aligned(q_out, 2))))
+      return fail(KVQ_ERR_ARG, "paged: k, v, q and q_out must be 2-byte aligned");
     a.k = static_cast<const uint16_t*>(k);
     a.val = static_cast<const uint16_t*>(v);
     a.k_row = k_strides[0];
