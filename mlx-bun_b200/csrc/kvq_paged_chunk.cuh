@@ -20,7 +20,10 @@
 // Roundings: K, V (as a dense cache of the dtype holds them) and the
 // probabilities go through the tensor core in the dtype; logits, statistics
 // and O are f32.  O is rescaled only when a row's maximum has grown by more
-// than 2^8 since the last time (p stays below 256, its sum in f32).
+// than 2^8 since the last time.  fp16 probabilities stand for 2^-7 of their value
+// (kLift: at most 2^15 with that growth), so that a key far below the row's
+// maximum keeps 2^-32 of it before it is lost: behind a first token that takes
+// the softmax, thousands of such keys are the output.
 //
 // Bound: per 128 keys and 256 rows at D 128 the tensor core needs 2048 clocks
 // (8192 dense flops a clock) and so do the exponentials (16 a clock per SM).
@@ -70,6 +73,11 @@ struct Chunk {
   static constexpr int PIECE = MR * (D + 2);    // floats: m [MR], l [MR], O [D / 4][MR][4]
   static_assert(SMEM <= 232448, "shared memory");
 };
+
+// log2 of what a probability is multiplied by before it is rounded; the sums
+// above and below the line carry it alike
+template <bool BF>
+constexpr float kLift = BF ? 0.0f : 7.0f;
 
 struct ChunkBars {
   uint64_t q_full[2], s_full[2], p_full[2], o_done[2];
@@ -441,8 +449,9 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         }
         mx = fmaxf(mx, other);
         mx = mx > 0.5f * kNeg ? mx * c2 : kNeg;
-        if (__any_sync(0xffffffffu, mx > m + 8.0f)) {  // the same for both halves
-          const float mn = fmaxf(m, mx), f = ex2(m - mn);
+        // the same for both halves; m is the reference, kLift below a maximum
+        if (__any_sync(0xffffffffu, mx > m + (8.0f + kLift<BF>))) {
+          const float mn = fmaxf(m, mx - kLift<BF>), f = ex2(m - mn);
           m = mn;
           l *= f;
           if (i > wk.i0) {

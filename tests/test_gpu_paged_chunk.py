@@ -53,3 +53,39 @@ def test_prefill_roundings(case, form):
     else:
         out, mag, magc, l1 = R.attention(ref, q, table, lens, cu, scale, window, sinks)
         _check(got, out, mag, magc, l1.abs(), dt)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16], ids=str)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_heavy_first_token_leaves_the_others_their_share(dt, bits, d):
+    """The first token takes nearly all of the softmax and brings nothing (v =
+    0); what the others bring, each with 2^-25.4 of its probability, is the whole
+    output.  Known in closed form: every other logit is 0 and every other v 1."""
+    hkv, hq, page, gs, n, rows = 8, 32, 64, 32, 16000, 1536
+    pages = n // page
+    ref = R.random_pool(torch.Generator().manual_seed(1), pages, page, hkv, d, gs, bits, dt)
+    ref.kp.zero_()
+    ref.vp.zero_()
+    ref.vp[..., 1] = 1.0
+    table = torch.arange(pages, dtype=torch.int32)[None]
+    # q is 1 in every element: the first key's logit is sum k * scale
+    ref.vp[0, :, 0, 0] = 0.0
+    k0 = 1.0
+    ref.kp[0, :, 0, 0, :, 1] = k0
+    x = 25.4 * float(np.log(2.0))
+    scale = x / (k0 * d)
+    cache = _cache(ref)
+    q = torch.ones(rows, hq, d, dtype=dt, device="cuda")
+    got = cache.sdpa_prefill(q, table.cuda(), _i32([n]), _i32([0, rows]), scale)
+    cache.check()
+    others = torch.arange(n - rows, n, dtype=torch.float64)
+    e = 2.0 ** -25.4
+    want = (others * e / (1 + others * e))[:, None, None]
+    # a probability's half step, fp16's subnormal steps of 2^-32 for each key, the
+    # logit (2^-18 of its 25 for the f32 sum, and 2^-24 of it for the scale), the output
+    u = R.half_step(dt)
+    tol = 2 * u * want + (others * 2.0 ** -32)[:, None, None] * (dt == F16) + 2 * (2.0 ** -18 * x) * want + \
+        (3e-8 if dt == F16 else 0)
+    err = (got.double().cpu() - want).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
