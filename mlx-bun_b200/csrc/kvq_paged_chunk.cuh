@@ -243,6 +243,23 @@ __device__ __forceinline__ constexpr int nib_pos(int i) { return (i >> 1) + (i &
 __device__ __forceinline__ uint32_t idesc_for(bool bf, int M, int N, int b_mn_major) {
   return attn::tc::idesc_f16(M, N, b_mn_major) | (bf ? (1u << 7) | (1u << 10) : 0u);
 }
+
+// n columns of a finished row to an `out` whose rows start anywhere, by element:
+// not inlined, since a branch in the usual loop costs the call 1 to 3 %.
+template <int BITS, bool BF>
+__device__ __noinline__ void store_any(uint32_t tO, uint16_t* dst, float inv, bool live, int n) {
+#pragma unroll 1
+  for (int d = 0; d < n; d += 8) {
+    uint32_t o[8];
+    attn::tc::tmem_ld8(tO + d, o);
+    attn::tc::tmem_wait_ld();
+    if (!live) continue;
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      dst[d + (BITS == 4 ? nib_pos(e) : e)] = attn::f_to_dt<BF>(__uint_as_float(o[e]) * inv);
+  }
+}
+
 template <int BITS, int D, int GS, bool BF>
 __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
     chunk_kernel(const AttnArgs a, const Work ws) {
@@ -543,8 +560,11 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
           }
         }
       }
+      const int d0 = half * (D / 2);
+      const bool apart = whole && a.out_align < 2;
+      if (apart) store_any<BITS, BF>(tm + lanes + C::TM_O + q * D + d0, dst + d0, inv, live, D / 2);
 #pragma unroll 1
-      for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 32) {
+      for (int d = d0; d < (apart ? d0 : d0 + D / 2); d += 32) {
         uint32_t o[32];
         tmem_ld32(tm + lanes + C::TM_O + q * D + d, o);
         tmem_wait_ld();
@@ -561,15 +581,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
               for (int i = 0; i < 4; i++)
                 w[i] = (uint32_t)attn::f_to_dt<BF>(x[e + 2 * i] * inv) |
                        ((uint32_t)attn::f_to_dt<BF>(x[e + 2 * i + 1] * inv) << 16);
-              if (a.out_align == 2) {
-                *reinterpret_cast<uint4*>(dst + d + e) = make_uint4(w[0], w[1], w[2], w[3]);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                  dst[d + e + 2 * i] = (uint16_t)w[i];
-                  dst[d + e + 2 * i + 1] = (uint16_t)(w[i] >> 16);
-                }
-              }
+              *reinterpret_cast<uint4*>(dst + d + e) = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
         } else {
