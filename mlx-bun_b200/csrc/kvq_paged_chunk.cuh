@@ -75,9 +75,10 @@ struct Chunk {
 };
 
 // log2 of what a probability is multiplied by before it is rounded; the sums
-// above and below the line carry it alike
+// above and below the line carry it alike.  bf16 has exponents to spare the other
+// way: 2^31 keys of V's largest value stay in range of the f32 sums.
 template <bool BF>
-constexpr float kLift = BF ? 0.0f : 7.0f;
+constexpr float kLift = BF ? -40.0f : 7.0f;
 
 struct ChunkBars {
   uint64_t q_full[2], s_full[2], p_full[2], o_done[2];
@@ -260,9 +261,114 @@ __device__ __noinline__ void store_any(uint32_t tO, uint16_t* dst, float inv, bo
   }
 }
 
+// Values that are not finite.  A row that does not see a key has p = 0 for it,
+// but 0 times an infinite V is not 0, so the tensor core gets finite ones only:
+// V that is not finite becomes 0 or the dtype's largest, and the rows that do
+// see such a pair are marked when they are written.  Finite pairs whose value
+// passes the dtype's range (the rounded scale times the last code does, in a row
+// of its largest values) count as the range's end, K and V alike.  A K pair that
+// is not finite stays: its logits are masked where they are hidden.
+template <bool BF>
+struct Range {
+  static constexpr uint32_t kInf = BF ? 0x7f80u : 0x7c00u;
+};
+
+// Whether a row's values are all finite and in range (bf16: below 2^127, to be
+// sure of the 8-bit codes' two roundings).  The last code's tells: a value is
+// monotone in its code, code 0 gives the bias, which is in range if it is finite,
+// and no finite value comes of a pair that is not.
+template <int BITS, int NG, bool BF>
+__device__ __forceinline__ bool pairs_in_range(const uint32_t (&pr)[NG]) {
+  constexpr uint32_t kLast = BF ? (BITS == 4 ? 0x41704170u : 0x437f437fu) : (BITS == 4 ? 0x4b804b80u : 0x5bf85bf8u);
+  constexpr uint32_t kStep = BF ? 0x01000100u : 0x04000400u;  // carries those exponents into the sign
+  uint32_t out = 0;
+#pragma unroll
+  for (int e = 0; e < NG; e += 2) {
+    const uint32_t other = pr[e + 1 < NG ? e + 1 : e];
+    const uint32_t s = prmt(pr[e], other, 0x5410u), z = prmt(pr[e], other, 0x7632u);
+    const uint32_t end = BF ? Dequant<BITS, BF>::fma_b(kLast, s, z) : Dequant<BITS, BF>::fma_h(kLast, s, z);
+    out |= (end & 0x7fff7fffu) + kStep;
+  }
+  return (out & 0x80008000u) == 0;
+}
+
+// One dequantized row in its swizzled panels, and its groups' pairs.  Not inlined:
+// the check and this call cost 512 rows over 16,896 keys 181 -> 183 us, inlined 186.
+template <int N>
+struct Pairs {
+  uint32_t w[N];
+};
+template <int D, int GS, int PANEL, bool BF>
+__device__ __noinline__ void hold_range(uint8_t* row, int r7, Pairs<D / GS> pr, bool is_v) {
+  uint32_t bad = 0;
+#pragma unroll
+  for (int e = 0; e < D / GS; e++)
+    if ((pr.w[e] & 0x7fffu) >= Range<BF>::kInf || ((pr.w[e] >> 16) & 0x7fffu) >= Range<BF>::kInf) bad |= 1u << e;
+  constexpr uint32_t kInf = Range<BF>::kInf;
+#pragma unroll 1
+  for (int e = 0; e < D / 8; e++) {
+    if (!is_v && ((bad >> (e * 8 / GS)) & 1u)) continue;
+    uint32_t* w = reinterpret_cast<uint32_t*>(row + (e >> 3) * PANEL + (((e & 7) ^ r7) << 4));
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const uint32_t x = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu, m = x & 0x7fffu;
+      if (m < kInf) continue;
+      const uint32_t y = m > kInf ? 0u : (x & 0x8000u) | (kInf - 1);
+      w[i >> 1] = (w[i >> 1] & ~(0xffffu << (16 * (i & 1)))) | (y << (16 * (i & 1)));
+    }
+  }
+}
+
+// The row at position p (of this lane; -1: none): NaN in its half of O wherever a
+// V pair that it sees in the segment is not finite.  A lane reads the pairs of
+// one key, every row takes those it sees.
+template <int BITS, int D, int GS, bool BF>
+__device__ __noinline__ void mark_lost(const AttnArgs& a, const Walk<BITS, D, GS>& wk, int p,
+                                       uint32_t tO, int half) {
+  using C = Chunk<BITS, D, GS>;
+  constexpr uint32_t kInf = Range<BF>::kInf;
+  const View& v = a.v;
+  const Block& k = wk.k;
+  const int lane = threadIdx.x & 31, klo = a.window > 0 ? max(0, k.pmin - a.window + 1) : 0;
+  const int32_t* table = v.table + (int64_t)k.b * v.table_stride;
+  uint32_t lost = 0;
+#pragma unroll 1
+  for (int n = 0; n < (wk.i1 - wk.i0) * (C::KT / 32); n++) {
+    const int j0 = (tile_of(k, wk.i0 + n / (C::KT / 32)) << C::KL) + n % (C::KT / 32) * 32, j = j0 + lane;
+    uint32_t bad = 0;
+    if (j <= k.pmax && (j >= klo || j < a.sinks)) {
+      const int page = table[j >> v.page_shift];
+      if (page >= 0 && page < v.num_pages) {
+        const uint8_t* src = tile_ptr(v, page, wk.h, (j & v.page_mask) >> 4) + C::HALF + kTileRows * C::CRB + (j & 15) * C::PRB;
+        for (int g = 0; g < D / GS; g++) {
+          const uint32_t pair = reinterpret_cast<const uint32_t*>(src)[g];
+          if ((pair & 0x7fffu) >= kInf || ((pair >> 16) & 0x7fffu) >= kInf) bad |= 1u << g;
+        }
+      }
+    }
+    for (uint32_t any = __ballot_sync(0xffffffffu, bad != 0); any; any &= any - 1) {
+      const int s = __ffs(any) - 1, jj = j0 + s;
+      const uint32_t x = __shfl_sync(0xffffffffu, bad, s);
+      if (jj <= p && (a.window == 0 || jj > p - a.window || jj < a.sinks)) lost |= x;
+    }
+  }
+#pragma unroll 1
+  for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 32) {
+    const bool hit = (lost >> (d / GS)) & 1u;
+    if (!__any_sync(0xffffffffu, hit)) continue;
+    uint32_t o[32];
+    attn::tc::tmem_ld32(tO + d, o);
+    attn::tc::tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 32; e++) o[e] = hit ? 0x7fc00000u : o[e];
+    attn::tc::tmem_st32(tO + d, o);
+    attn::tc::tmem_wait_st();
+  }
+}
+
 template <int BITS, int D, int GS, bool BF>
 __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
-    chunk_kernel(const AttnArgs a, const Work ws) {
+    chunk_kernel(const __grid_constant__ AttnArgs a, const Work ws) {
   using C = Chunk<BITS, D, GS>;
   using namespace attn::tc;
   constexpr int QT = C::QT, KB = C::KB, NG = D / GS;
@@ -275,6 +381,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
   volatile uint8_t* s_bad = sm + C::O_MISC + 16;  // [4 tiles in flight][4 warps]
   // [4]: what the MMA warp is to do with a tile (first / last of a segment)
   volatile int* s_what = reinterpret_cast<volatile int*>(sm + C::O_MISC + 32);
+  volatile int* s_lost = reinterpret_cast<volatile int*>(sm + C::O_MISC + 48);  // a V pair was not finite
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
@@ -291,6 +398,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       for (int w = 0; w < 8; w++) attn::mbar_init(&bar.x[w >> 2][w & 3][i], 64);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    *s_lost = 0;
   }
   if (warp == C::kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -538,6 +646,9 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         break;
       }
       l += rest;
+      // of any unit of the CTA so far; set before that tile's P V was issued
+      if (__any_sync(0xffffffffu, *s_lost))
+        mark_lost<BITS, D, GS, BF>(a, wk, p, tm + lanes + C::TM_O + q * D, half);
       const bool begun = wk.i0 == 0, ended = wk.i1 == k.nt, whole = begun && ended;
       const float inv = l != 0.0f ? 1.0f / l : 0.0f;
       const bool live = row < k.cols;
@@ -653,6 +764,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         j = key_of(n);
         page = page_of(j);
       }
+      const bool in_range = pairs_in_range<BITS, NG, BF>(pr);
       const int buf = KB == 2 ? tc & 1 : 0;
       // the buffer's last reader was tile tc - KB.  Four barriers by that tile's
       // number: a warp that had no V block for some tiles may be several releases
@@ -666,6 +778,13 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         const Dequant<BITS, BF> dq(pr[e * 8 / GS]);
         const uint32_t* words = reinterpret_cast<const uint32_t*>(raw) + e * BITS / 4;
         *reinterpret_cast<uint4*>(dst + (e >> 3) * C::PANEL + (((e & 7) ^ (r & 7)) << 4)) = dq.eight(words);
+      }
+      if (!in_range) {
+        Pairs<NG> all;
+#pragma unroll
+        for (int e = 0; e < NG; e++) all.w[e] = pr[e];
+        if (is_v) *s_lost = 1;
+        hold_range<D, GS, C::PANEL, BF>(dst, r & 7, all, is_v);
       }
       if (!is_v && lane == 0) {
         s_bad[(tc & 3) * 4 + quarter] = (uint8_t)(((lost & 0xffffu) ? 1 : 0) | ((lost >> 16) ? 2 : 0));
