@@ -13,18 +13,27 @@
 // code is the fp16 subnormal c 2^-24 (its bits in the low mantissa bits; 4-bit
 // codes of odd nibbles are taken unshifted as 16 c and the 16 is divided out
 // of q or of the output).  q is scaled by the power of two that brings its
-// largest element into [2^13, 2^14), so bf16 queries of any size and the
-// divided ones keep all their bits in fp16.  p_j s_j is rounded to fp16 (an
-// error of at most 2^-12 of it, times c); softmax statistics and all sums are
+// largest element into [2^13, 2^14), so bf16 queries between 2^-87 and 2^113 and
+// the divided ones keep all their bits in fp16.  p_j s_j is rounded to fp16 (an
+// error of at most 2^-11 of it, times c); softmax statistics and all sums are
 // f32.  For fp16 outputs that error is centred: with x_j the rounded p_j s_j
 // and h the middle code,
 //   sum_j x_j c_j - h sum_j x_j + sum_j p_j (z_j + h s_j),
 // so it multiplies c - h (half the range, 0 in the middle) instead of c; the
-// sum of x_j comes from one more MMA with ones.  The softmax reference m is a
-// running maximum of logit + floor(log2(largest |s| of the lane's rows))
-// rather than of the logit, so p_j s_j stays at most 2^5 and near one for the
-// keys that matter, whatever the size of V, and a single key's p is a power of
-// two, which rounds nothing.
+// sum of x_j comes from one more MMA with ones.
+//
+// Keeping p_j s_j in fp16's normal range, whatever the scales: the softmax
+// reference m of a column is a running maximum, over the keys it sees, of logit +
+// floor(log2(largest |s| of the key's row)) - kRaise rather than of the logit, so
+// p_j s_j reaches 2^15 and is normal down to 2^-24 of the terms that matter; and a
+// group whose scales lie below the others' is brought up to them by a power of
+// two of its own, in p_j s_j and its sums, divided out at the end.  Both are worked
+// out when a term passes the reference by more than 2^kLazy (always on the first
+// keys), from the keys at hand: a key that a column does not see has no say in
+// its reference, however large or not finite its scale.  Biases count by 2^-64 of
+// their size, which keeps sum p z in f32's range next to tiny scales.  Measured
+// against a reference by the lane's rows as a whole and without powers: 0 to 3 %
+// of the time of the forms of up to 8 columns, 1 to 12 % of those of 16.
 //
 // Bound: HBM.  4 bits, D 128, group 64: 144 B per key and kv head; at the
 // measured copy rate an SM gets 23 B per clock, one 16-key tile per 100
@@ -41,7 +50,7 @@
 // CTA, and otherwise in the merge kernel, always in order of the keys.
 //
 // Measured (B200): 64 ragged sequences of 1,024 to 32,768 keys, 8 kv heads, D
-// 128, 4 bits (1,050 MB): 197 us, 5.3 TB/s; 8 sequences of 8,193 keys: 26.3 us;
+// 128, 4 bits (1,050 MB): 197 us, 5.3 TB/s; 8 sequences of 8,193 keys: 26.6 us;
 // one of 2,048 keys in 8 bits: 11.3 us, all of it latency.
 #include <mutex>
 #include <set>
@@ -60,7 +69,10 @@ using attn::pack_h2;
 using attn::prmt;
 
 constexpr float kLazy = 4.0f;       // m moves when a term would exceed 2^4
-constexpr float kMinLogScale = -60.0f;
+constexpr float kMinScale = 8.673617379884035e-19f;  // 2^-60: the smallest that a reference goes by
+constexpr float kRaise = 10.0f;     // terms are at most 2^(kLazy + 1 + kRaise) = 2^15
+constexpr int kMaxUp = 30;          // most that a group is brought up, log2
+constexpr float kBiasShare = 5.421010862427522e-20f;  // 2^-64: p z stays in f32's range too
 constexpr int kPlanMax = 512;       // sequences and column blocks whose plan fits in shared memory
 
 // ------------------------------------------------------------- the plan --
@@ -229,8 +241,11 @@ struct Cfg {
   static constexpr int PIECE = 16 * NT + FR * 128;  // floats of a piece: m, l, O fragments
   // ring depth: a few KB in flight per warp; two stages of the large tiles
   static constexpr int STAGES = STAGE <= 5120 ? 3 : (STAGE <= 9216 && TPS == 1 ? 3 : 2);
-  // warps: what the registers allow (168 or 255 a thread), then shared memory
-  static constexpr int W_REG = D * NT <= 128 ? 12 : 8;
+  // warps: what the registers allow (168 or 255 a thread), then shared memory.
+  // Four groups in 4 bits at one column a lane spill at 168 (8 columns, 32
+  // sequences of 8,000 to 16,000 keys: 118 us with 8 warps, 135 with 12; in 8
+  // bits 149 and 137)
+  static constexpr int W_REG = D * NT > 128 || (BITS == 4 && D / GS >= 4 && ST == 1) ? 8 : 12;
   static constexpr int W_MEM = 224000 / (STAGES * STAGE + PIECE * 4);
   static constexpr int W = W_REG < W_MEM ? W_REG : W_MEM;
   static constexpr int PLAN_BYTES = (kPlanMax + 1) * 12 + 4;
@@ -240,7 +255,8 @@ struct Cfg {
   static constexpr int O_BAR = O_TMP + 33 * 8 + 8;
   static constexpr int O_META = O_BAR + W * STAGES * 8;
   static constexpr int O_INFO = (O_META + W * STAGES * TPS * 4 + 15) / 16 * 16;
-  static constexpr int SMEM = O_INFO + W * 2 * 16 + 128;
+  static constexpr int O_UP = O_INFO + W * 2 * 16;
+  static constexpr int SMEM = O_UP + W * (D / GS) * 4 + 128;
   static_assert(PIECE * 4 <= STAGES * STAGE, "a warp's last piece lies in its ring");
   static_assert(SMEM <= 232448, "shared memory");
   static_assert(ST == 1 || (ST == 2 && NT == 1), "two streams share one column tile");
@@ -270,6 +286,10 @@ struct State {
   int qp[NT][2];             // query position of the lane's columns
   float m[NT][2], l[NT][2], pz[NT][G::NG][2];
   float x1[NT][G::NG][4];    // sum of x per group (fp16 outputs)
+  // powers of two in x, o and x1 of each group, the same in all lanes; beyond two
+  // groups in shared memory, to spare registers
+  static constexpr bool kUpsHere = G::NG <= 2;
+  float up[kUpsHere ? G::NG : 1];
   float o[G::MT][NT][4];
 
   __device__ __forceinline__ void reset() {
@@ -348,10 +368,9 @@ __device__ __forceinline__ void load_q(State<BITS, D, GS, NT>& S, const AttnArgs
 #pragma unroll
       for (int w = 0; w < G::KW; w++)
 #pragma unroll
-        for (int i = 0; i < PW; i++) sum += x[gr][w][i];
+        for (int i = 0; i < PW; i++) sum = fmaf(x[gr][w][i], up, sum);
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      sum *= up;
       sum *= kUnit;
       S.qs[n][gr][0] = __shfl_sync(0xffffffffu, sum, (2 * t) << 2);
       S.qs[n][gr][1] = __shfl_sync(0xffffffffu, sum, (2 * t + 1) << 2);
@@ -400,11 +419,14 @@ __device__ __forceinline__ void load_pairs(float (&s)[NG], float (&z)[NG], const
   }
 }
 
+// 1 / x of a power of two
+__device__ __forceinline__ float pow2_inv(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
+
 // T tiles of a stage: keys j0[i]..j0[i] + 15.  MASK: some of them are not seen
 // by some column (or, j0 < 0, the tile was not there to be read): their
 // logits, scales and biases, whatever they hold, are replaced.
 template <int BITS, int D, int GS, int NT, int ST, bool BF, int T, bool MASK>
-__device__ __forceinline__ void process(State<BITS, D, GS, NT>& S, const uint8_t* st,
+__device__ __forceinline__ void process(State<BITS, D, GS, NT>& S, float* s_ups, const uint8_t* st,
                                         const int (&j0)[T], int window, int sinks, int g, int t) {
   using C = Cfg<BITS, D, GS, NT, ST>;
   using G = attn::Geo<BITS, D, GS>;
@@ -412,6 +434,7 @@ __device__ __forceinline__ void process(State<BITS, D, GS, NT>& S, const uint8_t
   constexpr int VT = ST == 2 ? 1 : T;  // sets of logits a lane holds
   constexpr float kMid = (float)((1 << BITS) - 1) * 0.5f;
   static_assert(ST == 1 || T == 2, "two streams take two tiles");
+  float* ups = State<BITS, D, GS, NT>::kUpsHere ? S.up : s_ups;
   const int ra = row_of(g);
   const bool up_stream = t >= 2;       // ST = 2: this lane's columns belong to tile 1
   float val[VT][NT][4];
@@ -473,31 +496,40 @@ __device__ __forceinline__ void process(State<BITS, D, GS, NT>& S, const uint8_t
       }
     }
   }
-  // V's scales and biases, and the exponent of the largest scale of the lane's rows
-  float vs[VT][2][NG], vz[VT][2][NG], big = 0.0f;
+  // V's scales (times the groups' powers) and biases.  A row counts towards the
+  // reference by the exponent of its largest scale, less kRaise; here the
+  // largest of all of the lane's rows stands for each
+  const uint8_t* vp = st + (ST == 2 && up_stream ? C::TILE : 0) + C::HALF + kTileRows * C::CRB + ra * C::PRB;
+  float vs[VT][2][NG], vz[VT][2][NG];
+  auto load_v = [&]() {
 #pragma unroll
-  for (int i = 0; i < VT; i++) {
-    const uint8_t* vp = st + (ST == 2 ? (up_stream ? C::TILE : 0) : i * C::TILE) + C::HALF +
-                        kTileRows * C::CRB;
+    for (int i = 0; i < VT; i++)
 #pragma unroll
-    for (int r = 0; r < 2; r++) {
-      load_pairs<NG, BF>(vs[i][r], vz[i][r], vp + (ra + 8 * r) * C::PRB);
-      bool any = !MASK;
-      if constexpr (MASK) {
+      for (int r = 0; r < 2; r++) {
+        load_pairs<NG, BF>(vs[i][r], vz[i][r], vp + i * C::TILE + 8 * r * C::PRB);
 #pragma unroll
-        for (int n = 0; n < NT; n++) any = any || see[i][n][2 * r] || see[i][n][2 * r + 1];
+        for (int gr = 0; gr < NG; gr++) {
+          if constexpr (!BF) vz[i][r][gr] = fmaf(kMid, vs[i][r][gr], vz[i][r][gr]);
+          vs[i][r][gr] *= ups[gr];
+        }
       }
+  };
+  // 2^23 + the exponent field, by its bits
+  auto exponent = [&](float x) {
+    return __uint_as_float(__funnelshift_r(__float_as_uint(x), 0x4b000000u >> 9, 23)) - (8388608.0f + 127.0f + kRaise);
+  };
+  load_v();
+  float big = kMinScale, big_z = 0.0f;
+#pragma unroll
+  for (int i = 0; i < VT; i++)
+#pragma unroll
+    for (int r = 0; r < 2; r++)
 #pragma unroll
       for (int gr = 0; gr < NG; gr++) {
-        if (any) big = fmaxf(big, fabsf(vs[i][r][gr]));
-        if constexpr (!BF) vz[i][r][gr] = fmaf(kMid, vs[i][r][gr], vz[i][r][gr]);
+        big = fmaxf(big, fabsf(vs[i][r][gr]));
+        if constexpr (BF) big_z = fmaxf(big_z, fabsf(vz[i][r][gr]));
       }
-    }
-  }
-  float lsm;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lsm) : "f"(__int_as_float(__float_as_int(big) & 0x7f800000)));
-  lsm = fmaxf(lsm, kMinLogScale);
-  float mx[NT][2];
+  const float most_exp = exponent(BF ? fmaxf(big, big_z * kBiasShare) : big);
   bool up = false;
 #pragma unroll
   for (int n = 0; n < NT; n++)
@@ -506,15 +538,66 @@ __device__ __forceinline__ void process(State<BITS, D, GS, NT>& S, const uint8_t
       float x = fmaxf(val[0][n][c], val[0][n][c + 2]);
 #pragma unroll
       for (int i = 1; i < VT; i++) x = fmaxf(x, fmaxf(val[i][n][c], val[i][n][c + 2]));
-      mx[n][c] = x + lsm;
-      up = up || mx[n][c] > S.m[n][c] + kLazy;
+      up = up || x + most_exp > S.m[n][c] + kLazy;
     }
   if (__any_sync(0xffffffffu, up)) {
+    // the groups' powers anew: each brings its largest scale in the rows that
+    // are seen up to the largest of all.  What is not finite has no say.  (Pairs
+    // are read again one at a time: held over this, they cost spills.)
+    asm volatile("" ::: "memory");
+    auto pair = [&](int i, int r, int gr) {
+      return *reinterpret_cast<const uint32_t*>(vp + i * C::TILE + 8 * r * C::PRB + 4 * gr);
+    };
+    uint32_t most[NG], all = 0;
+    float grow[NG], row_exp[VT][2];
+#pragma unroll
+    for (int gr = 0; gr < NG; gr++) {
+      uint32_t e = 0;
+#pragma unroll
+      for (int i = 0; i < VT; i++)
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          bool any = !MASK;
+          if constexpr (MASK) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) any = any || see[i][n][2 * r] || see[i][n][2 * r + 1];
+          }
+          const uint32_t x = __float_as_uint(fabsf(attn::dt_to_f<BF>((uint16_t)pair(i, r, gr))));
+          if (any && x < 0x7f800000u) e = max(e, x);
+        }
+      most[gr] = __reduce_max_sync(0xffffffffu, e) >> 23;
+      all = max(all, most[gr]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int gr = 0; gr < NG; gr++) {
+      const float now = __uint_as_float((127u + min(all - most[gr], (uint32_t)kMaxUp)) << 23);
+      grow[gr] = now * pow2_inv(ups[gr]);
+      ups[gr] = now;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < VT; i++)
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        float x = kMinScale;
+#pragma unroll
+        for (int gr = 0; gr < NG; gr++) {
+          const uint32_t w = pair(i, r, gr);
+          const float y = fabsf(attn::dt_to_f<BF>((uint16_t)w)) * ups[gr];
+          const float z = BF ? fabsf(attn::dt_to_f<BF>((uint16_t)(w >> 16))) * kBiasShare : 0.0f;
+          x = fmaxf(x, fmaxf(y < INFINITY ? y : 0.0f, z < INFINITY ? z : 0.0f));
+        }
+        row_exp[i][r] = exponent(x);
+      }
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        float x = mx[n][c];
+        float x = fmaxf(val[0][n][c] + row_exp[0][0], val[0][n][c + 2] + row_exp[0][1]);
+#pragma unroll
+        for (int i = 1; i < VT; i++)
+          x = fmaxf(x, fmaxf(val[i][n][c] + row_exp[i][0], val[i][n][c + 2] + row_exp[i][1]));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -524,15 +607,18 @@ __device__ __forceinline__ void process(State<BITS, D, GS, NT>& S, const uint8_t
         S.l[n][c] *= f;
 #pragma unroll
         for (int gr = 0; gr < NG; gr++) {
+          const float fg = f * grow[gr];
           S.pz[n][gr][c] *= f;
-          if constexpr (!BF) S.x1[n][gr][c] *= f;
-        }
+          if constexpr (!BF) S.x1[n][gr][c] *= fg;
 #pragma unroll
-        for (int k = 0; k < G::MT; k++) {
-          S.o[k][n][c] *= f;
-          S.o[k][n][c + 2] *= f;
+          for (int k = gr * G::MTG; k < (gr + 1) * G::MTG; k++) {
+            S.o[k][n][c] *= fg;
+            S.o[k][n][c + 2] *= fg;
+          }
         }
       }
+    asm volatile("" ::: "memory");
+    load_v();
   }
 #pragma unroll
   for (int i = 0; i < VT; i++) {
@@ -631,7 +717,8 @@ __device__ __forceinline__ void store_out(const AttnArgs& a, const Block& k, int
 // Close a segment: sums over the lanes of a column, outputs in natural units,
 // the two streams joined.
 template <int BITS, int D, int GS, int NT, int ST, bool BF>
-__device__ __forceinline__ void close(State<BITS, D, GS, NT>& S) {
+__device__ __forceinline__ void close(State<BITS, D, GS, NT>& S, const float* s_ups) {
+  const float* ups = State<BITS, D, GS, NT>::kUpsHere ? S.up : s_ups;
   using G = attn::Geo<BITS, D, GS>;
   constexpr float kMid = (float)((1 << BITS) - 1) * 0.5f;
 #pragma unroll
@@ -647,10 +734,11 @@ __device__ __forceinline__ void close(State<BITS, D, GS, NT>& S) {
       }
 #pragma unroll
       for (int k = 0; k < G::MT; k++) {
-        constexpr float odd = BITS == 4 ? attn::kCodeUnitInv * 0.0625f : attn::kCodeUnitInv;
+        const float down = pow2_inv(ups[k / G::MTG]), unit = attn::kCodeUnitInv * down;
+        const float odd = BITS == 4 ? unit * 0.0625f : unit;
         float add = S.pz[n][k / G::MTG][c];
-        if constexpr (!BF) add = fmaf(-kMid, S.x1[n][k / G::MTG][c], add);
-        S.o[k][n][c] = fmaf(S.o[k][n][c], attn::kCodeUnitInv, add);
+        if constexpr (!BF) add = fmaf(-kMid * down, S.x1[n][k / G::MTG][c], add);
+        S.o[k][n][c] = fmaf(S.o[k][n][c], unit, add);
         S.o[k][n][c + 2] = fmaf(S.o[k][n][c + 2], odd, add);
       }
       if constexpr (ST == 2) {
@@ -821,7 +909,16 @@ __global__ void __launch_bounds__(Cfg<BITS, D, GS, NT, ST>::W * 32, 1)
     for (int s = 0; s < STAGES; s++) issue();
 
     State<BITS, D, GS, NT> S;
+    float* ups = reinterpret_cast<float*>(smem + C::O_UP) + w * G::NG;
+    auto start_ups = [&]() {
+      __syncwarp();
+      if (lane < G::NG) ups[lane] = 1.0f;
+#pragma unroll
+      for (float& x : S.up) x = 1.0f;
+      __syncwarp();
+    };
     S.reset();
+    start_ups();
     load_q<BITS, D, GS, NT, ST, BF>(S, a, kc, hc, ws.vec, g, t);
     bool begun = ic == 0;  // this segment holds the unit's first tile
     int stage = 0;
@@ -851,10 +948,10 @@ __global__ void __launch_bounds__(Cfg<BITS, D, GS, NT, ST>::W * 32, 1)
           bad |= j0[i];
         }
         if (ic >= fa && ic + TPS <= fb && bad >= 0) {
-          process<BITS, D, GS, NT, ST, BF, TPS, false>(S, st, j0, a.window, a.sinks, g, t);
+          process<BITS, D, GS, NT, ST, BF, TPS, false>(S, ups, st, j0, a.window, a.sinks, g, t);
         } else {
           if (TPS == 2 && ic + 1 == e) j0[TPS - 1] = -1;
-          process<BITS, D, GS, NT, ST, BF, TPS, true>(S, st, j0, a.window, a.sinks, g, t);
+          process<BITS, D, GS, NT, ST, BF, TPS, true>(S, ups, st, j0, a.window, a.sinks, g, t);
         }
         __syncwarp();
         issue();
@@ -867,7 +964,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, GS, NT, ST>::W * 32, 1)
       ic = e;
 
       // the segment ends: the unit is done, or the warp's run is
-      close<BITS, D, GS, NT, ST, BF>(S);
+      close<BITS, D, GS, NT, ST, BF>(S, ups);
       const bool ended = ic == kc.nt;
       const int unit = gi * v.Hkv + hc;
       if (begun && ended) {
@@ -912,6 +1009,7 @@ __global__ void __launch_bounds__(Cfg<BITS, D, GS, NT, ST>::W * 32, 1)
           kc = get_block<NC>(a, P, gi);
         }
         S.reset();
+        start_ups();
         load_q<BITS, D, GS, NT, ST, BF>(S, a, kc, hc, ws.vec, g, t);
         begun = true;
       }

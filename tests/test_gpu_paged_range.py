@@ -5,7 +5,7 @@ import torch
 
 import paged_chunk_ref as C
 import paged_ref as R
-from test_gpu_paged import _cache, _cu, _i32, _pages
+from test_gpu_paged import _cache, _check, _cu, _i32, _pages
 
 pytestmark = pytest.mark.gpu
 
@@ -23,6 +23,139 @@ def _row(ref, table, b, pos):
     """Index of position `pos` of sequence b in the pool's parts (all heads)."""
     pg, tile, row = ref.index(table[b], torch.tensor([pos]))
     return int(pg), slice(None), int(tile), int(row)
+
+
+def _check_after_first(got, ref, q, table, lens, cu, scale, dt, window=0, sinks=0):
+    """_check, for rows of which the first of a sequence may see nothing."""
+    for b, n in enumerate(lens):
+        skip = max(0, cu[b + 1] - cu[b] - n)
+        r0, r1 = cu[b] + skip, cu[b + 1]
+        assert not got[cu[b]:r0].any()
+        want = R.attention(ref, q[r0:r1], table[b:b + 1], [n], [0, r1 - r0], scale, window, sinks)
+        _check(got[r0:r1], *want, dt)
+
+
+# ------------------------------------------------------- few rows a sequence --
+
+FORMS = [
+    # Hq, Hkv, D, gs, rows of each sequence (None: single tokens)
+    (8, 2, 128, 64, None), (16, 2, 128, 64, None), (16, 1, 128, 32, None), (8, 2, 64, 32, None),
+    (4, 2, 256, 64, None), (16, 2, 256, 128, None), (8, 2, 128, 32, [3, 2, 4, 1]),
+]
+
+
+@pytest.mark.parametrize("dt", [F16, BF16], ids=str)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("form", FORMS, ids=lambda f: "-".join(str(x) for x in f[:4]) + ("" if f[4] is None else "-rows"))
+@pytest.mark.parametrize("apart", ["zero", 10, 14, 18, 40])
+def test_groups_of_v_far_apart(dt, bits, form, apart):
+    """One group of every V row far below the others (or all zeros, as the
+    append leaves it) keeps its own precision."""
+    if apart == 40 and dt == F16:
+        pytest.skip("fp16 has no such scale")
+    hq, hkv, d, gs, rows = form
+    lens = [2048, 700, 33, 1]
+    gen, ref, table = _pool(41, lens, 16, hkv, d, gs, bits, dt)
+    low = d // gs - 1
+    if apart == "zero":
+        ref.vp[..., 0] *= 64.0
+        ref.vp[..., 1] *= 64.0
+        ref.vp[..., low, 0] = 1e-7
+        ref.vp[..., low, 1] = 0.0
+        w = gs * bits // 32
+        ref.vc[..., low * w:(low + 1) * w] = 0
+    else:
+        ref.vp[..., low, :] *= 2.0 ** -apart
+    cache = _cache(ref)
+    cu = _cu(rows or [1] * 4)
+    q = torch.randn(cu[-1], hq, d, generator=gen).to(dt)
+    if rows is None:
+        got = cache.sdpa_decode(q.cuda(), table.cuda(), _i32(lens), d ** -0.5)
+    else:
+        got = cache.sdpa_prefill(q.cuda(), table.cuda(), _i32(lens), _i32(cu), d ** -0.5)
+    cache.check()
+    _check_after_first(got, ref, q, table, lens, cu, d ** -0.5, dt)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16], ids=str)
+@pytest.mark.parametrize("hq", [8, 16])
+def test_a_heavy_first_token_with_a_small_v(dt, hq):
+    """The first token takes the softmax and brings a V 2^-9 of the others',
+    which together bring as much: neither may be rounded away."""
+    B, n, hkv, d, gs, bits = 48, 4000, 2, 128, 64, 8
+    lens = [n] * B
+    pages = -(-n // 64)
+    gen = torch.Generator().manual_seed(42)
+    ref = R.random_pool(gen, pages, 64, hkv, d, gs, bits, dt)
+    table = torch.arange(pages, dtype=torch.int32)[None].expand(B, -1).contiguous()  # one prefix for all
+    first = (0, slice(None), 0, 0)
+    ref.kp[..., 0] *= 0.25
+    ref.kp[..., 1] = (-ref.kp[..., 0].double() * 127.5).to(dt)
+    ref.kp[first][..., 0] = 0.0
+    ref.kp[first][..., 1] = 1.0      # logit: sum of q * scale
+    ref.vp[first] = ref.vp[first] * 2.0 ** -9
+    scale = 25.0 * 0.6931472 / d     # 2^25 for a q of ones
+    q = (1.0 + 0.05 * torch.randn(B, hq, d, generator=gen)).to(dt)
+    cache = _cache(ref)
+    got = cache.sdpa_decode(q.cuda(), table.cuda(), _i32(lens), scale)
+    cache.check()
+    want = R.attention(ref, q[:4], table[:4], lens[:4], list(range(5)), scale)
+    _check(got[:4], *want, dt)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16], ids=str)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hq", [2, 4, 16])
+@pytest.mark.parametrize("what", ["huge", "inf scale", "nan scale", "inf bias"])
+def test_drafts_do_not_feel_later_keys(dt, bits, hq, what):
+    """The last row's own key has a V scale far above the others', or one that
+    is not finite: the rows before it do not see it."""
+    hkv, d, gs, n, rows = 2, 128, 64, 45, 4
+    gen, ref, table = _pool(43, [n], 16, hkv, d, gs, bits, dt)
+    at = _row(ref, table, 0, n - 1)
+    if what == "huge":
+        ref.vp[..., :] *= 2.0 ** -9
+        ref.vp[at] = ref.vp[at] * (2.0 ** 20 if dt == F16 else 2.0 ** 60)
+    else:
+        ref.vp[at][..., 1, 1 if what == "inf bias" else 0] = float("nan" if what == "nan scale" else "inf")
+    cache = _cache(ref)
+    q = torch.randn(rows, hq, d, generator=gen).to(dt)
+    got = cache.sdpa_prefill(q.cuda(), table.cuda(), _i32([n]), _i32([0, rows]), 0.09)
+    cache.check()
+    want = R.attention(ref, q[:-1], table, [n - 1], [0, rows - 1], 0.09)
+    _check(got[:-1], *want, dt)
+    last = R.attention(ref, q[-1:], table, [n], [0, 1], 0.09)
+    if what == "huge":
+        _check(got[-1:], *last, dt)
+    else:  # the group with the bad pair is not finite, the other is right
+        assert not torch.isfinite(got[-1:, :, gs:]).any()
+        _check(got[-1:, :, :gs], *[x[..., :gs] for x in last], dt)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_constant_rows_near_the_largest_bf16(bits):
+    """Groups of one huge value have the smallest scale and a huge bias."""
+    lens, d = [300, 20], 128
+    gen, ref, table = _pool(44, lens, 16, 2, d, 64, bits, BF16)
+    ref.vp[..., 0] = 1e-7
+    ref.vp[..., 1] = 1e37
+    ref.vp[:, 1, ..., 1] *= -1.0
+    cache = _cache(ref)
+    q = torch.randn(2, 8, d, generator=gen).to(BF16)
+    got = cache.sdpa_decode(q.cuda(), table.cuda(), _i32(lens), 0.09)
+    cache.check()
+    _check(got, *R.attention(ref, q, table, lens, [0, 1, 2], 0.09), BF16)
+
+
+def test_queries_near_the_largest_bf16():
+    lens, d = [200, 64], 128
+    gen, ref, table = _pool(45, lens, 16, 2, d, 64, 8, BF16)
+    ref.kp *= 2.0 ** -110
+    cache = _cache(ref)
+    q = (1.0 + 0.3 * torch.randn(2, 8, d, generator=gen)).to(BF16) * 2.0 ** 108
+    got = cache.sdpa_decode(q.cuda(), table.cuda(), _i32(lens), 0.1)
+    cache.check()
+    _check(got, *R.attention(ref, q, table, lens, [0, 1, 2], 0.1), BF16)
 
 
 # ------------------------------------------------------------- prompt chunks --
