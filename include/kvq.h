@@ -500,9 +500,11 @@ int32_t kvq_paged_sdpa_prefill(const kvq_paged* cache, const kvq_paged_batch* ba
                                float scale, int32_t window, int32_t sinks, void* out,
                                void* workspace, size_t workspace_bytes, void* stream);
 
-/* Synchronize `stream`, report (then clear) the pool's error flag:
- * KVQ_ERR_STATE for a row, page or length that made no sense, KVQ_ERR_CUDA for a
- * bounded wait in a kernel that ran out. */
+/* Synchronize `stream`, take (read and clear in one step) the pool's error flag
+ * and report it: KVQ_ERR_STATE for a row, page or length that made no sense,
+ * KVQ_ERR_CUDA for a bounded wait in a kernel that ran out.  The flag belongs to
+ * the pool: calls on other streams raise the same one, and what they raise later
+ * stays for a later check. */
 int32_t kvq_paged_check(const kvq_paged* cache, void* stream);
 
 /* ---- context split across the GPUs of one node (peer memory) ----------- */

@@ -141,6 +141,10 @@ int32_t sdpa(const kvq_paged* c, const kvq_paged_batch* b, bool decode, const vo
   return rc;
 }
 
+// Reads and clears the error flag in one step: a kernel of another stream may
+// raise it at any time, and what it raises after this is the next check's.
+__global__ void take_status(int* status, int* taken) { *taken = atomicExch(status, 0); }
+
 // No exception leaves a C entry (bookkeeping maps and messages allocate).
 template <class F>
 int32_t guarded(F&& f) noexcept {
@@ -268,12 +272,21 @@ int32_t kvq_paged_check(const kvq_paged* c, void* stream) {
     if (!c || !c->status) return fail(KVQ_ERR_ARG, "paged: NULL cache / status");
     DeviceGuard guard(c->device);
     if (!guard.ok) return fail(KVQ_ERR_CUDA, "cannot select the cache's device");
-    KVQ_CUDA_TRY(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    KVQ_CUDA_TRY(cudaStreamSynchronize(st));
     int flag = 0;
-    KVQ_CUDA_TRY(cudaMemcpy(&flag, c->status, sizeof(int), cudaMemcpyDeviceToHost));
+    cudaMemPool_t pool = nullptr;
+    int32_t rc = scratch_pool(c->device, &pool);
+    if (rc) return rc;
+    int* taken = nullptr;
+    KVQ_CUDA_TRY(cudaMallocFromPoolAsync(reinterpret_cast<void**>(&taken), sizeof(int), pool, st));
+    take_status<<<1, 1, 0, st>>>(c->status, taken);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaMemcpyAsync(&flag, taken, sizeof(int), cudaMemcpyDeviceToHost, st);
+    const cudaError_t f = cudaFreeAsync(taken, st), w = cudaStreamSynchronize(st);
+    for (cudaError_t x : {e, f, w})
+      if (x != cudaSuccess) return cuda_fail(x, "kvq_paged_check");
     if (!flag) return KVQ_OK;
-    const int zero = 0;
-    KVQ_CUDA_TRY(cudaMemcpy(c->status, &zero, sizeof(int), cudaMemcpyHostToDevice));
     if (flag & 2) return fail(KVQ_ERR_CUDA, "a paged kernel gave up waiting (its results are not valid)");
     return fail(KVQ_ERR_STATE,
                 "a paged call met a row without a place, a page number outside the pool or a length "

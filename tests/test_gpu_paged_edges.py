@@ -74,3 +74,43 @@ def test_out_may_start_at_any_element(case, cut):
     cache.check()
     assert torch.equal(out.view(torch.int16), want.view(torch.int16))
     assert (buf[:cut] == 7.0).all() and (buf[cut + n * hq * d:] == 7.0).all()
+
+
+# ------------------------------------------------------- streams and the flag --
+
+def _small(seed=32, n=40):
+    gen = torch.Generator().manual_seed(seed)
+    ref = R.random_pool(gen, 6, 16, 2, 64, 64, 4, F16)
+    table = R.make_table(gen, [n], 16, 6)
+    return gen, ref, table, _cache(ref)
+
+
+def test_check_takes_what_is_raised_by_then():
+    """Errors are reported once, by the first check after them; one that another
+    stream raises later is the next check's."""
+    kvq = _kvq()
+    gen, ref, table, cache = _small()
+    k = torch.randn(1, 2, 64, generator=gen).to(F16).cuda()
+    good, bad = _i32([40]), _i32([4000])  # a position past the table
+    dtab = table.cuda()
+    cache.append(k, k, dtab, bad)
+    with pytest.raises(kvq.KvqError):
+        cache.check()
+    cache.check()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s2):
+        torch.cuda._sleep(200_000_000)  # about 0.1 s
+        cache.append(k, k, dtab, bad)
+    with torch.cuda.stream(s1):
+        cache.append(k, k, dtab, good)
+        cache.check()               # nothing of s1's; s2 has not come to its append
+    with torch.cuda.stream(s2):
+        with pytest.raises(kvq.KvqError):
+            cache.check()
+    with torch.cuda.stream(s1):
+        cache.check()
+    cache._status.fill_(3)          # both kinds at once: the wait that ran out is told
+    with pytest.raises(kvq.KvqError, match="waiting"):
+        cache.check()
+    cache.check()
