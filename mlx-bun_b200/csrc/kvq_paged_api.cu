@@ -89,9 +89,16 @@ int32_t scratch_pool(int dev, cudaMemPool_t* out) {
     props.location.type = cudaMemLocationTypeDevice;
     props.location.id = dev;
     cudaMemPool_t pool = nullptr;
-    KVQ_CUDA_TRY(cudaMemPoolCreate(&pool, &props));
+    // the first call may be one that is being captured, where a pool cannot be
+    // made otherwise
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    KVQ_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
     uint64_t keep = UINT64_MAX;
-    KVQ_CUDA_TRY(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep));
+    cudaError_t e = cudaMemPoolCreate(&pool, &props);
+    if (e == cudaSuccess) e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
+    const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMemPoolCreate");
+    if (back != cudaSuccess) return cuda_fail(back, "cudaThreadExchangeStreamCaptureMode");
     g_pool[dev] = pool;
   }
   *out = g_pool[dev];

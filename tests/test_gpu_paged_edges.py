@@ -114,3 +114,48 @@ def test_check_takes_what_is_raised_by_then():
     with pytest.raises(kvq.KvqError, match="waiting"):
         cache.check()
     cache.check()
+
+
+CAPTURE = """
+import torch, sys
+sys.path[:0] = [%r, %r]
+import kvq, paged_ref as R
+import test_gpu_paged_edges as T
+gen, ref, table, cache = T._small()
+q = torch.randn(3, 8, 64, generator=gen).to(torch.float16).cuda()
+lens, cu, dtab = T._i32([38]), T._i32([0, 3]), table.cuda()
+kw = dict(window=20, sinks=2)
+out = [torch.zeros_like(q) for _ in range(2)]
+out1 = torch.zeros(1, 8, 64, dtype=torch.float16, device="cuda")
+side = torch.cuda.Stream()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=side):
+    for o in out:  # the library's own workspaces, of a stream that is being captured
+        cache.sdpa_prefill(q, dtab, lens, cu, 0.1, out=o, stream=side.cuda_stream, **kw)
+    cache.sdpa_decode(q[2:], dtab, lens, 0.1, out=out1, stream=side.cuda_stream, **kw)
+for n in (38, 40, 35):
+    lens.fill_(n)
+    for o in out + [out1]:
+        o.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    cache.check()
+    want = cache.sdpa_prefill(q, dtab, lens, cu, 0.1, **kw)
+    assert torch.equal(out[0], want) and torch.equal(out[1], want)
+    assert torch.equal(out1, cache.sdpa_decode(q[2:], dtab, lens, 0.1, **kw))
+print("captured")
+"""
+
+
+def test_capture_with_the_librarys_workspaces():
+    """The first call of a process that needs the library's own memory may come
+    while its stream is being captured."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = CAPTURE % (here, os.path.join(os.path.dirname(here), "mlx-bun_b200"))
+    env = dict(os.environ, PYTHONPATH=os.path.dirname(here))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, env=env)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
