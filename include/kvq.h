@@ -468,8 +468,9 @@ int32_t kvq_paged_tile_bytes(const kvq_paged* cache, size_t* bytes);
  * kv_heads, head_dim] dtype with element strides (row, head); the element
  * stride is 1.  q (nullable): device [rows, q_heads, head_dim] with its own
  * strides, whose rotated rows go to q_out (contiguous [rows, q_heads,
- * head_dim], or q itself when q is contiguous).  rope NULL: no rotation.  Two
- * rows of one step must not share a position of one page. */
+ * head_dim], or q itself when q is contiguous; otherwise apart from q, k and
+ * v).  rope NULL: no rotation.  Two rows of one step must not share a position
+ * of one page. */
 int32_t kvq_paged_append(const kvq_paged* cache, const kvq_paged_batch* batch, const void* k,
                          const void* v, const int64_t* k_strides, const int64_t* v_strides,
                          const kvq_rope* rope, const void* q, int32_t q_heads,
@@ -477,10 +478,11 @@ int32_t kvq_paged_append(const kvq_paged* cache, const kvq_paged_batch* batch, c
 
 /* Causal attention of the step's query rows over their sequences' pages.
  * q: device [rows, q_heads, head_dim] with element strides (row, head); out:
- * contiguous [rows, q_heads, head_dim], at any element of its buffer; query
- * head h uses kv head h / (q_heads / kv_heads).  A query at position p sees key j when j <= p and (window == 0
- * or j > p - window or j < sinks): a sliding window with the first `sinks`
- * tokens kept visible.  A row that sees no key gives zeros.  k and v are code
+ * contiguous [rows, q_heads, head_dim], at any element of its buffer (q itself
+ * when q is contiguous, otherwise apart from q); query head h uses kv head h /
+ * (q_heads / kv_heads).  A query at position p sees key j when j <= p and
+ * (window == 0 or j > p - window or j < sinks): a sliding window with the first
+ * `sinks` tokens kept visible.  A row that sees no key gives zeros.  k and v are code
  * * scale + bias, logits and softmax are f32, the output is rounded once.
  * kvq_paged_sdpa_decode takes one row per sequence (cu_rows is not read,
  * rows = batch); kvq_paged_sdpa_prefill takes ragged rows.

@@ -15,6 +15,25 @@ namespace {
 // does): the kernels load whole elements.
 bool aligned(const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
 
+// Whether the contiguous rows that a call writes at `out` share memory with the
+// rows [rows][heads][D] it reads at `in` (element strides rs, hs).
+bool shares(const void* out, const void* in, int64_t rows, int64_t heads, int64_t D, int64_t out_heads,
+            int64_t rs, int64_t hs) {
+  if (rs < 0) {
+    in = static_cast<const uint16_t*>(in) + (rows - 1) * rs;
+    rs = -rs;
+  }
+  const int64_t a = reinterpret_cast<intptr_t>(out), b = a + rows * out_heads * D * 2, len = 2 * D, step = 2 * rs;
+  for (int64_t h = 0; h < heads; h++) {
+    const int64_t x = reinterpret_cast<intptr_t>(in) + 2 * h * hs;  // rows at x + r * step, len bytes each
+    if (x >= b) continue;
+    // the first row that ends behind a
+    const int64_t r = x + len > a ? 0 : step ? (a - (x + len)) / step + 1 : rows;
+    if (r < rows && x + r * step < b) return true;
+  }
+  return false;
+}
+
 int32_t make_view(const kvq_paged* c, const kvq_paged_batch* b, paged::View& v) {
   if (!c || !b) return fail(KVQ_ERR_ARG, "paged: NULL cache / batch");
   if (!c->pool || !c->status) return fail(KVQ_ERR_ARG, "paged: NULL pool / status");
@@ -118,6 +137,9 @@ int32_t sdpa(const kvq_paged* c, const kvq_paged_batch* b, bool decode, const vo
   if (a.v.rows == 0 || a.v.B == 0) return KVQ_OK;
   if (!q || !q_strides || !out) return fail(KVQ_ERR_ARG, "paged: NULL q / q_strides / out");
   if (!aligned(q, 2) || !aligned(out, 2)) return fail(KVQ_ERR_ARG, "paged: q and out must be 2-byte aligned");
+  const bool packed = (q_heads == 1 || q_strides[1] == a.v.D) && (a.v.rows == 1 || q_strides[0] == (int64_t)q_heads * a.v.D);
+  if (!(out == q && packed) && shares(out, q, a.v.rows, q_heads, a.v.D, q_heads, q_strides[0], q_strides[1]))
+    return fail(KVQ_ERR_ARG, "paged: out overlaps q (it may be q itself when q is contiguous)");
   a.q = static_cast<const uint16_t*>(q);
   a.q_row = q_strides[0];
   a.q_head = q_strides[1];
@@ -220,6 +242,10 @@ int32_t kvq_paged_append(const kvq_paged* c, const kvq_paged_batch* b, const voi
     if (!k || !v || !k_strides || !v_strides) return fail(KVQ_ERR_ARG, "paged: NULL k / v / strides");
     if (!aligned(k, 2) || !aligned(v, 2) || (q && (!aligned(q, 2) || !aligned(q_out, 2))))
       return fail(KVQ_ERR_ARG, "paged: k, v, q and q_out must be 2-byte aligned");
+    if (q && (shares(q_out, k, a.v.rows, a.v.Hkv, a.v.D, q_heads, k_strides[0], k_strides[1]) ||
+              shares(q_out, v, a.v.rows, a.v.Hkv, a.v.D, q_heads, v_strides[0], v_strides[1]) ||
+              (q_out != q && shares(q_out, q, a.v.rows, q_heads, a.v.D, q_heads, q_strides[0], q_strides[1]))))
+      return fail(KVQ_ERR_ARG, "paged: q_out overlaps k, v or (other than as q itself) q");
     a.k = static_cast<const uint16_t*>(k);
     a.val = static_cast<const uint16_t*>(v);
     a.k_row = k_strides[0];

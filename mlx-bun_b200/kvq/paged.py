@@ -161,9 +161,9 @@ class PagedQuantizedKVCache:
         head strides) into their pages: K rotated by `rope` at its position,
         both quantized (kvq_paged_append).  q [rows, q_heads, head_dim]: its
         rotated rows go to q_out (allocated when None; q itself to rotate a
-        contiguous q in place), which is returned.  Padding rows (from
-        cu_rows[batch] on) are not touched: a fresh q_out holds anything
-        there."""
+        contiguous q in place, otherwise apart from q, k and v), which is
+        returned.  Padding rows (from cu_rows[batch] on) are not touched: a
+        fresh q_out holds anything there."""
         shape, ks = self._rows(k, "k", self.kv_heads)
         vshape, vs = self._rows(v, "v", self.kv_heads)
         rows = shape[0]
@@ -224,7 +224,8 @@ class PagedQuantizedKVCache:
                     stream=None) -> torch.Tensor:
         """Attention of one query row per sequence, q [batch, q_heads,
         head_dim], at the sequences' last positions (kvq_paged_sdpa_decode).
-        window > 0: the last `window` keys and the first `sinks` ones.
+        window > 0: the last `window` keys and the first `sinks` ones.  `out`
+        may be a contiguous q itself, otherwise lies apart from it.
         workspace None: the call's own, safe with calls on other streams."""
         return self._sdpa(lib().kvq_paged_sdpa_decode, q, page_table, seq_lens, None, scale, window,
                           sinks, out, workspace, stream)

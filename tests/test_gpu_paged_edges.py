@@ -76,6 +76,30 @@ def test_out_may_start_at_any_element(case, cut):
     assert (buf[:cut] == 7.0).all() and (buf[cut + n * hq * d:] == 7.0).all()
 
 
+@pytest.mark.parametrize("case", OUT, ids=lambda c: "-".join(str(x) for x in c[1:]))
+def test_out_may_be_q(case):
+    dt, bits, gs, hq, hkv, d, page, lens, rows = case
+    gen = torch.Generator().manual_seed(33)
+    ref = R.random_pool(gen, _pages(lens, page), page, hkv, d, gs, bits, dt)
+    table = R.make_table(gen, lens, page, ref.pool.shape[0]).cuda()
+    cache = _cache(ref)
+    n = len(lens) if rows is None else sum(rows)
+    q = torch.randn(n, hq, d, generator=gen).to(dt).cuda()
+
+    def call(q, out=None):
+        if rows is None:
+            return cache.sdpa_decode(q, table, _i32(lens), 0.1, out=out)
+        return cache.sdpa_prefill(q, table, _i32(lens), _i32(_cu(rows)), 0.1, out=out)
+
+    want = call(q)
+    for _ in range(5):
+        x = q.clone()
+        assert torch.equal(call(x, x).view(torch.int16), want.view(torch.int16))
+    with pytest.raises(_kvq().KvqError, match="overlaps"):
+        buf = torch.zeros((n + 1) * hq * d, dtype=dt, device="cuda")
+        call(buf[:n * hq * d].view(n, hq, d), buf[hq:hq + n * hq * d].view(n, hq, d))
+
+
 # ------------------------------------------------------- streams and the flag --
 
 def _small(seed=32, n=40):
