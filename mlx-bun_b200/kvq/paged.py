@@ -209,6 +209,8 @@ class PagedQuantizedKVCache:
             key = (cu_rows is None, shape[0], batch.batch, shape[1])
             wsb = self._ws_bytes.get(key)
             if wsb is None:
+                if len(self._ws_bytes) >= 4096:  # a server meets ever new counts of rows
+                    self._ws_bytes.clear()
                 wsb = self._ws_bytes[key] = self._workspace(batch, shape[1], cu_rows is None)
             workspace = torch.empty(wsb, dtype=torch.uint8, device=self.device)
             ws = workspace.data_ptr()

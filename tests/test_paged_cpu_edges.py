@@ -95,3 +95,25 @@ def test_queries_that_are_not_contiguous_are_not_rotated_or_answered_in_place():
     for qs in (_strides(WIDE + 8, 128), _strides(WIDE, 64), _strides(0, 128)):
         rc = fn(ctypes.byref(paged()), ctypes.byref(batch()), A, 8, qs, 1.0, 0, 0, A, None, 0, None)
         assert rc == _lib.ERR_ARG and "overlaps" in error()
+
+
+def test_remembered_workspace_sizes_are_bounded():
+    """A server whose steps bring ever new counts of rows."""
+    import torch
+
+    import kvq
+    cache = object.__new__(kvq.PagedQuantizedKVCache)
+    cache._index, cache.device, cache.dtype, cache.head_dim = -1, torch.device("cpu"), torch.float16, 64
+    cache._ref, cache._ws_bytes = None, {}
+    asked = []
+    cache._stream = lambda stream: 0
+    cache._workspace = lambda batch, heads, decode: asked.append(batch.rows) or 16
+    lens, cu = torch.zeros(1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    table = torch.zeros(1, 1, dtype=torch.int32)
+    buf = torch.zeros(9000, 1, 64, dtype=torch.float16)
+    call = lambda n: cache._sdpa(lambda *a: 0, buf[:n], table, lens, cu, 1.0, 0, 0, buf[:n], None, None)
+    for n in range(9000):
+        call(n)
+        call(n)  # known by now
+    assert asked == list(range(9000))
+    assert len(cache._ws_bytes) <= 4096
