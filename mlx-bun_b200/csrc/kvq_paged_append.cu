@@ -28,6 +28,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxHalf = 128;
 constexpr int kMaxRows = 4;  // rows of a block
+constexpr int kSms = 148;    // of a B200
 
 template <bool BF>
 __device__ __forceinline__ float to_f(uint16_t v) {
@@ -412,15 +413,20 @@ bool vec_ok(const void* p, int64_t row, int64_t head) {
 
 template <bool BF, int BITS, int GS>
 int32_t launch(bool vec, cudaStream_t st, const AppendArgs& a) {
-  // few rows: one unit per thread, so that a step's latency is one pass; many:
-  // four to a block, whose angles then keep all its threads busy
+  // Few rows: one unit per thread (up to two blocks an SM, 296), so that a step's
+  // latency is one pass; many: four rows to a block, whose angles then keep all
+  // its threads busy, from eight rows an SM (148) on.  us, three shapes (32 + 8
+  // heads x 128 in 4 bits, 16 + 8 x 256 in 8, 8 + 2 x 64 in 4): 16 rows split /
+  // not split 3.4 / 4.2, 4.1 / 5.9, 3.2 / 3.2; one row a block / four: 592 rows
+  // 7.4 / 8.5, 10.4 / 13.9, 4.0 / 5.5; 1,184 rows 12.6 / 11.3, 19.1 / 22.2, 6.6 /
+  // 6.0; 1,776 rows 18.1 / 14.8, 27.5 / 23.1, 9.4 / 6.2.
   const int units = (2 * a.v.Hkv + (a.q ? a.Hq : 0)) * a.v.D / 8;
   int parts = 1;
-  while (parts < (units + kThreads - 1) / kThreads && (int64_t)a.v.rows * parts < 296) parts++;
+  while (parts < (units + kThreads - 1) / kThreads && (int64_t)a.v.rows * parts < 2 * kSms) parts++;
   const dim3 grid((unsigned)a.v.rows, (unsigned)parts), block(kThreads);
   if (!vec)
     KVQ_CUDA_TRY(launch_pdl(append_any_kernel<BF, BITS, GS>, grid, block, 0, st, a));
-  else if (a.v.rows < 148 * 8)
+  else if (a.v.rows < 8 * kSms)
     KVQ_CUDA_TRY(launch_pdl(append_kernel<BF, BITS, GS, 1>, grid, block, 0, st, a));
   else
     KVQ_CUDA_TRY(launch_pdl(append_kernel<BF, BITS, GS, kMaxRows>,

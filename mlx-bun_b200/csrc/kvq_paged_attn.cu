@@ -28,7 +28,12 @@ int32_t launch_chunk<8, true>(const AttnArgs&, const Work&, int, int, cudaStream
 namespace {
 
 // Query rows (times heads of a group) per sequence above which a call goes to
-// the chunk kernel.
+// the chunk kernel: a mean over the call, since rows of single sequences are known
+// on the GPU only.  The two cross between 32 and 130 (us at 32, 64, 128 columns,
+// column kernel / chunk kernel): 16 sequences of 8,000 keys, D 128, 4
+// bits: 107 / 164, 194 / 165, 366 / 169; one, 8 bits: 21 / 41, 27 / 42, 42 / 43; 4
+// of 4,000, D 256, 8 bits: 58 / 61, 100 / 63, 183 / 66; 8 of 4,000, D 64, 4 bits:
+// 22 / 35, 29 / 35, 42 / 36.
 constexpr long long kChunkCols = 64;
 
 size_t up16(size_t x) { return (x + 15) / 16 * 16; }

@@ -32,7 +32,7 @@
 // the pieces of a cut unit (m, l, O in f32) meet in the merge kernel in order.
 //
 // Measured (B200): 512 rows over 16,896 keys, 32 query and 8 kv heads, D 128, 8
-// bits (139.6 GFLOP): 181 us, 771 TFLOP/s, about 5,000 clocks a tile.  D 256, two
+// bits (139.6 GFLOP): 183 us, 763 TFLOP/s, about 5,000 clocks a tile.  D 256, two
 // chunks of up to 1,024 rows, window 1,024, 8 bits: 110 us; one K / V buffer of 128
 // keys instead of two of 64 took 133.
 #include "kvq_paged_cols.cuh"
@@ -47,7 +47,7 @@ struct Chunk {
   static constexpr int MR = 128 * QT;
   static constexpr int KL = D == 256 ? 6 : 7, KT = 1 << KL;  // keys per tile: 64 or 128
   static constexpr int NBK = KT / 32, BL = KL - 4;  // 32-row blocks of K; log2 of K's and V's
-  static constexpr int KB = 2;                  // K (and V) buffers
+  static constexpr int KB = 2;                  // K (and V) buffers, taken by a tile's parity
   static constexpr int QPANEL = 128 * 128;      // bytes: 128 rows of 64 elements
   static constexpr int QTILE = D / 64 * QPANEL;
   static constexpr int PANEL = KT * 128;        // the same of a K or V tile
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
     chunk_kernel(const __grid_constant__ AttnArgs a, const Work ws) {
   using C = Chunk<BITS, D, GS>;
   using namespace attn::tc;
-  constexpr int QT = C::QT, KB = C::KB, NG = D / GS;
+  constexpr int QT = C::QT, NG = D / GS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = smem_raw + ((1024 - (attn::smem_u32(smem_raw) & 1023)) & 1023);
   const View& v = a.v;
@@ -765,11 +765,11 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
         page = page_of(j);
       }
       const bool in_range = pairs_in_range<BITS, NG, BF>(pr);
-      const int buf = KB == 2 ? tc & 1 : 0;
-      // the buffer's last reader was tile tc - KB.  Four barriers by that tile's
+      const int buf = tc & 1;
+      // the buffer's last reader was tile tc - 2.  Four barriers by that tile's
       // number: a warp that had no V block for some tiles may be several releases
       // behind, which fewer barriers' parities cannot tell apart.
-      const int was = tc - KB;
+      const int was = tc - C::KB;
       if (was >= 0 && !wait_all(is_v ? &bar.v_empty[was & 3] : &bar.k_empty[was & 3], (was >> 2) & 1)) break;
       const int r = quarter * 32 + lane;
       uint8_t* dst = sm + (is_v ? C::O_V : C::O_K) + buf * C::TILE + (r >> 3) * 1024 + (r & 7) * 128;
@@ -805,7 +805,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
     // The whole warp runs this role, so that addresses and descriptors stay in
     // uniform registers; one elected lane issues.
     auto qk = [&](int q, int t) {  // S of row tile q, tile t
-      const int buf = KB == 2 ? t & 1 : 0;
+      const int buf = t & 1;
       const uint32_t dS = tm + (QT == 2 ? q : t & 1) * 128;
       if (!elect_one()) return;
 #pragma unroll
@@ -816,7 +816,7 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
       umma_commit(&bar.s_full[QT == 2 ? q : t & 1]);
     };
     auto pv = [&](int q, int t, bool first) {
-      const int buf = KB == 2 ? t & 1 : 0;
+      const int buf = t & 1;
       const uint32_t tP = tm + (QT == 2 ? q : t & 1) * 128;
       if (!elect_one()) return;
 #pragma unroll
@@ -828,8 +828,8 @@ __global__ void __launch_bounds__(Chunk<BITS, D, GS>::kThreads, 1)
     auto commit = [&](uint64_t* b) {
       if (elect_one()) umma_commit(b);
     };
-    auto kwait = [&](int t) { return wait_all(&bar.k_full[KB == 2 ? t & 1 : 0], (KB == 2 ? t >> 1 : t) & 1); };
-    auto vwait = [&](int t) { return wait_all(&bar.v_full[KB == 2 ? t & 1 : 0], (KB == 2 ? t >> 1 : t) & 1); };
+    auto kwait = [&](int t) { return wait_all(&bar.k_full[t & 1], (t >> 1) & 1); };
+    auto vwait = [&](int t) { return wait_all(&bar.v_full[t & 1], (t >> 1) & 1); };
     // A tile's products S are issued before the turn of its predecessor's P V
     // ends; `what` says when that predecessor belongs to another unit.
     auto start = [&](int t, int u) {  // the first tile of a segment

@@ -1,7 +1,7 @@
 #pragma once
 // kvq_paged_cols.cuh — attention of a few query rows per sequence over the
-// pages: single-token decode, drafted tokens, and chunks of shapes that the
-// tensor-memory kernel does not take.
+// pages: single-token decode, drafted tokens, and ragged steps of few rows a
+// sequence on average.
 //
 // Mathematics.  A unit is one (sequence, kv head) and up to 8 * NT of its
 // query columns (column c is token c / rep, head c % rep of the group), so a
