@@ -482,10 +482,24 @@ int32_t kvq_paged_append(const kvq_paged* cache, const kvq_paged_batch* batch, c
  * when q is contiguous, otherwise apart from q); query head h uses kv head h /
  * (q_heads / kv_heads).  A query at position p sees key j when j <= p and
  * (window == 0 or j > p - window or j < sinks): a sliding window with the first
- * `sinks` tokens kept visible.  A row that sees no key gives zeros.  k and v are code
- * * scale + bias, logits and softmax are f32, the output is rounded once.
+ * `sinks` tokens kept visible.  A row that sees no key gives zeros.
  * kvq_paged_sdpa_decode takes one row per sequence (cu_rows is not read,
  * rows = batch); kvq_paged_sdpa_prefill takes ragged rows.
+ * Precision: k and v are code * scale + bias, softmax statistics and all sums
+ * are f32, the output is rounded once.  What goes through the tensor cores in
+ * 16 bits depends on the call:
+ *   few rows (every kvq_paged_sdpa_decode, and kvq_paged_sdpa_prefill up to rows
+ *   * q_heads / kv_heads = 64 * batch, where rows counts the whole buffer with its
+ *   padding): K is exact, the probability times V's scale is rounded to fp16;
+ *   many rows: K, V and the probabilities are rounded to the dtype, as with a
+ *   dense cache of it; code * scale + bias past its range counts as its end.
+ * RMS error against 64 bits, relative to the output's: few rows 2.6e-4 (fp16)
+ * and 1.7e-3 (bf16), many rows 5.5e-4 and 3.4e-3; the output's own rounding is
+ * 2.1e-4 and 1.7e-3 of it.  So a row's last bits may differ with what else the
+ * call holds.
+ * A key that a row does not see has no effect on it, whatever its scales and
+ * biases hold.  Where a row sees a V scale or bias that is not finite, the
+ * group's outputs are not finite; a K one spoils the row.
  * workspace: device memory of kvq_paged_sdpa_workspace bytes (16-byte
  * aligned, contents irrelevant) that no other call uses meanwhile; NULL: the
  * call takes and returns its own, stream-ordered (cudaMallocFromPoolAsync, from

@@ -50,8 +50,8 @@
 // CTA, and otherwise in the merge kernel, always in order of the keys.
 //
 // Measured (B200): 64 ragged sequences of 1,024 to 32,768 keys, 8 kv heads, D
-// 128, 4 bits (1,050 MB): 197 us, 5.3 TB/s; 8 sequences of 8,193 keys: 26.6 us;
-// one of 2,048 keys in 8 bits: 11.3 us, all of it latency.
+// 128, 4 bits (1,050 MB): 197 us, 5.3 TB/s; 8 sequences of 8,193 keys: 26.7 us;
+// one of 2,048 keys in 8 bits: 11.5 us, all of it latency.
 #include <mutex>
 #include <set>
 

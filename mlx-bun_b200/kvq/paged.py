@@ -239,7 +239,10 @@ class PagedQuantizedKVCache:
         """Causal attention of ragged query rows, q [rows, q_heads, head_dim]:
         sequence b's rows are cu_rows[b]..cu_rows[b + 1] and end at its last
         position (kvq_paged_sdpa_prefill).  Padding rows are not touched: a
-        fresh `out` holds anything there."""
+        fresh `out` holds anything there.  Beyond rows * q_heads / kv_heads = 64
+        * batch (rows of the buffer, padding included) K, V and the
+        probabilities are rounded to the dtype before their products; below, K
+        is exact, as in sdpa_decode (errors: include/kvq.h)."""
         return self._sdpa(lib().kvq_paged_sdpa_prefill, q, page_table, seq_lens, cu_rows, scale,
                           window, sinks, out, workspace, stream)
 
