@@ -490,7 +490,9 @@ int32_t kvq_paged_append(const kvq_paged* cache, const kvq_paged_batch* batch, c
  * 16 bits depends on the call:
  *   few rows (every kvq_paged_sdpa_decode, and kvq_paged_sdpa_prefill up to rows
  *   * q_heads / kv_heads = 64 * batch, where rows counts the whole buffer with its
- *   padding): K is exact, the probability times V's scale is rounded to fp16;
+ *   padding): K is exact, the probability times V's scale is rounded to fp16
+ *   (in its normal range for groups of V up to 2^39 apart, which fp16 scales
+ *   always are);
  *   many rows: K, V and the probabilities are rounded to the dtype, as with a
  *   dense cache of it; code * scale + bias past its range counts as its end.
  * RMS error against 64 bits, relative to the output's: few rows 2.6e-4 (fp16)

@@ -31,9 +31,13 @@
 // out when a term passes the reference by more than 2^kLazy (always on the first
 // keys), from the keys at hand: a key that a column does not see has no say in
 // its reference, however large or not finite its scale.  Biases count by 2^-64 of
-// their size, which keeps sum p z in f32's range next to tiny scales.  Measured
-// against a reference by the lane's rows as a whole and without powers: 0 to 3 %
-// of the time of the forms of up to 8 columns, 1 to 12 % of those of 16.
+// their size, which keeps sum p z in f32's range next to tiny scales.  The powers
+// are the same for all columns and at most 2^20 (kMaxUp): a group 2^39 below the
+// reference's, or left 2^20 behind by the powers of columns that see more, still
+// has its largest term at 2^-5, 2^20 above fp16's last bit.  fp16 scales span 2^37;
+// bf16 ones of groups of neighbouring keys may lie 2^39 apart.  Measured against a
+// reference by the lane's rows as a whole and without powers: 0 to 3 % of the
+// time of the forms of up to 8 columns, 1 to 12 % of those of 16.
 //
 // Bound: HBM.  4 bits, D 128, group 64: 144 B per key and kv head; at the
 // measured copy rate an SM gets 23 B per clock, one 16-key tile per 100
@@ -71,7 +75,7 @@ using attn::prmt;
 constexpr float kLazy = 4.0f;       // m moves when a term would exceed 2^4
 constexpr float kMinScale = 8.673617379884035e-19f;  // 2^-60: the smallest that a reference goes by
 constexpr float kRaise = 10.0f;     // terms are at most 2^(kLazy + 1 + kRaise) = 2^15
-constexpr int kMaxUp = 30;          // most that a group is brought up, log2
+constexpr int kMaxUp = 20;          // most that a group is brought up, log2 (half of what fp16 scales span)
 constexpr float kBiasShare = 5.421010862427522e-20f;  // 2^-64: p z stays in f32's range too
 constexpr int kPlanMax = 512;       // sequences and column blocks whose plan fits in shared memory
 
@@ -514,6 +518,14 @@ __device__ __forceinline__ void process(State<BITS, D, GS, NT>& S, float* s_ups,
         }
       }
   };
+  auto any_sees = [&](int i, int r) {
+    bool any = !MASK;
+    if constexpr (MASK) {
+#pragma unroll
+      for (int n = 0; n < NT; n++) any = any || see[i][n][2 * r] || see[i][n][2 * r + 1];
+    }
+    return any;
+  };
   // 2^23 + the exponent field, by its bits
   auto exponent = [&](float x) {
     return __uint_as_float(__funnelshift_r(__float_as_uint(x), 0x4b000000u >> 9, 23)) - (8388608.0f + 127.0f + kRaise);
@@ -523,12 +535,14 @@ __device__ __forceinline__ void process(State<BITS, D, GS, NT>& S, float* s_ups,
 #pragma unroll
   for (int i = 0; i < VT; i++)
 #pragma unroll
-    for (int r = 0; r < 2; r++)
+    for (int r = 0; r < 2; r++) {
+      if (!any_sees(i, r)) continue;  // (whatever lies there must not change a bit)
 #pragma unroll
       for (int gr = 0; gr < NG; gr++) {
         big = fmaxf(big, fabsf(vs[i][r][gr]));
         if constexpr (BF) big_z = fmaxf(big_z, fabsf(vz[i][r][gr]));
       }
+    }
   const float most_exp = exponent(BF ? fmaxf(big, big_z * kBiasShare) : big);
   bool up = false;
 #pragma unroll
@@ -557,13 +571,8 @@ __device__ __forceinline__ void process(State<BITS, D, GS, NT>& S, float* s_ups,
       for (int i = 0; i < VT; i++)
 #pragma unroll
         for (int r = 0; r < 2; r++) {
-          bool any = !MASK;
-          if constexpr (MASK) {
-#pragma unroll
-            for (int n = 0; n < NT; n++) any = any || see[i][n][2 * r] || see[i][n][2 * r + 1];
-          }
           const uint32_t x = __float_as_uint(fabsf(attn::dt_to_f<BF>((uint16_t)pair(i, r, gr))));
-          if (any && x < 0x7f800000u) e = max(e, x);
+          if (any_sees(i, r) && x < 0x7f800000u) e = max(e, x);
         }
       most[gr] = __reduce_max_sync(0xffffffffu, e) >> 23;
       all = max(all, most[gr]);
@@ -601,7 +610,8 @@ __device__ __forceinline__ void process(State<BITS, D, GS, NT>& S, float* s_ups,
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-        x = fmaxf(x, S.m[n][c]);
+        // only where its own keys pass it: what moved another column stays there
+        x = x > S.m[n][c] + kLazy ? x : S.m[n][c];
         const float f = ex2(S.m[n][c] - x);
         S.m[n][c] = x;
         S.l[n][c] *= f;

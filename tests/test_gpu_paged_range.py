@@ -106,7 +106,7 @@ def test_a_heavy_first_token_with_a_small_v(dt, hq):
 @pytest.mark.parametrize("dt", [F16, BF16], ids=str)
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("hq", [2, 4, 16])
-@pytest.mark.parametrize("what", ["huge", "inf scale", "nan scale", "inf bias"])
+@pytest.mark.parametrize("what", ["huge", "huge group", "inf scale", "nan scale", "inf bias"])
 def test_drafts_do_not_feel_later_keys(dt, bits, hq, what):
     """The last row's own key has a V scale far above the others', or one that
     is not finite: the rows before it do not see it."""
@@ -116,6 +116,11 @@ def test_drafts_do_not_feel_later_keys(dt, bits, hq, what):
     if what == "huge":
         ref.vp[..., :] *= 2.0 ** -9
         ref.vp[at] = ref.vp[at] * (2.0 ** 20 if dt == F16 else 2.0 ** 60)
+    elif what == "huge group":
+        ref.vp[..., :] *= 2.0 ** -9
+        # groups of neighbouring keys may lie 2^39 apart: fp16 scales always do (2^-24
+        # to 2^13), 2^36 is left for bf16 next to scales that differ by up to 3
+        ref.vp[at][..., 1, :] *= 2.0 ** 20 if dt == F16 else 2.0 ** 36
     else:
         ref.vp[at][..., 1, 1 if what == "inf bias" else 0] = float("nan" if what == "nan scale" else "inf")
     cache = _cache(ref)
@@ -125,7 +130,7 @@ def test_drafts_do_not_feel_later_keys(dt, bits, hq, what):
     want = R.attention(ref, q[:-1], table, [n - 1], [0, rows - 1], 0.09)
     _check(got[:-1], *want, dt)
     last = R.attention(ref, q[-1:], table, [n], [0, 1], 0.09)
-    if what == "huge":
+    if "huge" in what:
         _check(got[-1:], *last, dt)
     else:  # the group with the bad pair is not finite, the other is right
         assert not torch.isfinite(got[-1:, :, gs:]).any()
@@ -238,3 +243,54 @@ def test_chunks_of_values_at_the_end_of_the_range(bits, d, dt):
     for n in ("out", "mag", "sq", "l1", "keys"):
         setattr(want, n, getattr(want, n)[keep])
     want.check(got[keep.cuda()], dt)
+
+
+# ----------------------------------------------------- what nobody is to see --
+
+HIDDEN = [
+    # Hq, Hkv, D, gs, lens, rows (None: single tokens), window, sinks
+    (8, 2, 128, 64, [1000, 17, 333, 5], None, 0, 0),
+    (16, 2, 128, 32, [700, 33], None, 100, 3),
+    (16, 1, 64, 32, [555, 70], None, 0, 0),
+    (8, 2, 256, 64, [300, 41], None, 50, 0),
+    (8, 2, 128, 64, [200, 90], [5, 3], 40, 2),
+    (8, 2, 128, 64, [400, 190], [300, 130], 100, 5),
+    (4, 2, 256, 32, [500, 100], [200, 100], 0, 0),
+    # enough for a warp to meet several tiles of a sequence
+    (32, 8, 128, 64, [300 + 37 * i % 600 for i in range(56)], None, 0, 0),
+    (64, 8, 64, 32, [300 + 37 * i % 600 for i in range(56)], None, 0, 0),
+    (16, 8, 128, 32, [300 + 37 * i % 600 for i in range(56)], [1 + i % 5 for i in range(56)], 150, 2),
+]
+
+
+@pytest.mark.parametrize("dt", [F16, BF16], ids=str)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("case", HIDDEN, ids=lambda c: "-".join(str(x) for x in c)[:48])
+def test_rows_that_nobody_sees_do_not_change_a_bit(dt, bits, case):
+    """The rows behind a sequence's end, and those that its window has left, hold
+    zeros, ordinary, huge or no numbers."""
+    hq, hkv, d, gs, lens, rows, window, sinks = case
+    gen, ref, table = _pool(48, lens, 16, hkv, d, gs, bits, dt)
+    seen = torch.zeros(ref.kc.shape[0], ref.kc.shape[2], 16, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        j = torch.arange(n)
+        first = n - (1 if rows is None else rows[b])
+        keep = j[(j < sinks) | (j > first - window)] if window else j
+        seen[ref.index(table[b], keep)] = True
+    hidden = ~seen[:, None, :, :, None, None]
+    cu = _cu(rows or [1] * len(lens))
+    q = torch.randn(cu[-1], hq, d, generator=gen).to(dt).cuda()
+    results = []
+    for what in (0.0, 1.0, -1.0, torch.finfo(dt).max, float("inf"), float("nan")):
+        other = R.RefPool(ref.pool, 16, hkv, d, gs, bits, dt)
+        for p in (other.kp, other.vp):
+            p.copy_(torch.where(hidden.expand_as(p), torch.full_like(p, what), p))
+        cache = _cache(other)
+        for _ in range(2):
+            if rows is None:
+                got = cache.sdpa_decode(q, table.cuda(), _i32(lens), 0.1, window, sinks)
+            else:
+                got = cache.sdpa_prefill(q, table.cuda(), _i32(lens), _i32(cu), 0.1, window, sinks)
+            results.append(got.view(torch.int16).cpu())
+        cache.check()
+    assert all(torch.equal(r, results[0]) for r in results)
