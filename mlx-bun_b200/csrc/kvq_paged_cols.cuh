@@ -576,12 +576,13 @@ __device__ __forceinline__ void process(State<BITS, D, GS, NT>& S, float* s_ups,
         }
       most[gr] = __reduce_max_sync(0xffffffffu, e) >> 23;
       all = max(all, most[gr]);
+      grow[gr] = pow2_inv(ups[gr]);
     }
-    __syncwarp();
+    __syncwarp();  // every lane has read them
 #pragma unroll
     for (int gr = 0; gr < NG; gr++) {
       const float now = __uint_as_float((127u + min(all - most[gr], (uint32_t)kMaxUp)) << 23);
-      grow[gr] = now * pow2_inv(ups[gr]);
+      grow[gr] *= now;
       ups[gr] = now;
     }
     __syncwarp();
