@@ -495,10 +495,11 @@ int32_t kvq_paged_append(const kvq_paged* cache, const kvq_paged_batch* batch, c
  *   always are);
  *   many rows: K, V and the probabilities are rounded to the dtype, as with a
  *   dense cache of it; code * scale + bias past its range counts as its end.
- * RMS error against 64 bits, relative to the output's: few rows 2.6e-4 (fp16)
- * and 1.7e-3 (bf16), many rows 5.5e-4 and 3.4e-3; the output's own rounding is
- * 2.1e-4 and 1.7e-3 of it.  So a row's last bits may differ with what else the
- * call holds.
+ * RMS error against 64 bits, relative to the output's, on normal data: few rows
+ * 2.6e-4 (fp16) and 1.7e-3 (bf16), many rows 5.5e-4 and 3.4e-3 (at most 2.9e-4,
+ * 2.0e-3, 6.9e-4 and 5.3e-3 over 3,353 drawn shapes); the output's own rounding
+ * is 2.1e-4 and 1.7e-3 of it.  So a row's last bits may differ with what else
+ * the call holds.
  * A key that a row does not see has no effect on it, whatever its scales and
  * biases hold.  Where a row sees a V scale or bias that is not finite, the
  * group's outputs are not finite; a K one spoils the row.
